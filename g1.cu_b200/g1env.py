@@ -60,6 +60,10 @@ SIGNATURES = {
     "g1_obs_prep": (ctypes.c_int, [ctypes.c_longlong, ctypes.c_int] + [_vp] * 6),
     "g1_adv_normalize": (ctypes.c_int, [ctypes.c_longlong, _vp, _vp, _vp]),
     "g1_runnorm_update": (ctypes.c_int, [ctypes.c_int, _vp, _vp, ctypes.c_double, _vp, _vp]),
+    "g1_opt_workspace": (ctypes.c_longlong, [ctypes.c_int]),
+    "g1_clip_grad_norm": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp, ctypes.c_double, _vp, _vp, ctypes.c_longlong, _vp]),
+    "g1_clip_adam": (ctypes.c_int, [ctypes.c_int] + [_vp] * 7 + [ctypes.c_double, ctypes.c_double, _vp]
+                     + [ctypes.c_double] * 4 + [_vp, _vp, ctypes.c_longlong, _vp]),
     "g1_qacc_batch": (ctypes.c_int, [ctypes.c_int] + [_vp] * 4 + [ctypes.c_int, ctypes.c_float] + [_vp] * 5),
 }
 
@@ -330,6 +334,173 @@ def runnorm_update_device(norm, obs_mom, rows_total):
                              _stream()):
         _check()
     norm.count = norm.count + rows_total
+
+
+# ---------------- gradient norm, clipping and the clipped Adam step ----------------
+_GRAD_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _on(dev):
+    """Makes `dev` the current device for the calls within (nothing where it is already)."""
+    return torch.cuda.device(dev)
+
+
+def _dense(t):
+    """Whether t fills its memory without gaps, in whatever order of its axes."""
+    if t.is_contiguous():
+        return True
+    order = sorted(range(t.dim()), key=t.stride, reverse=True)
+    return t.permute(order).is_contiguous()
+
+
+def _cuda_list(tensors, what, types):
+    dev = None
+    for t in tensors:
+        if not t.is_cuda:
+            raise G1Error(f"{what} must be CUDA tensors")
+        if dev is None:
+            dev = t.device
+        if t.device != dev:
+            raise G1Error(f"{what} must be on one device")
+        if t.dtype not in types:
+            raise G1Error(f"{what} must be {' / '.join(str(x)[6:] for x in types)}, not {str(t.dtype)[6:]}")
+        if not _dense(t):
+            raise G1Error(f"{what} must fill their memory without gaps (use .contiguous())")
+    return dev
+
+
+def _ptrs(tensors):
+    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+def clip_grad_norm_device(grads, max_norm):
+    """The global 2-norm over all tensors of `grads` (a tensor or an iterable of fp32 / bf16 / fp16 CUDA tensors; the
+    types may differ), and grads *= min(1, max_norm / (norm + 1e-6)) in place (g1_clip_grad_norm), on torch's
+    current stream.  Returns the norm before clipping as a CUDA fp32 scalar; nothing synchronises.  The
+    squares are summed in fp64 in a fixed order.  A norm that is NaN or infinite scales as in
+    torch.nn.utils.clip_grad_norm_.  Tensors of one call may not share memory."""
+    _require_gpu()
+    lib = load_library()
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    dev = _cuda_list(grads, "gradients", _GRAD_TYPE)
+    if dev is None:
+        dev = torch.device("cuda", torch.cuda.current_device())
+    n = len(grads)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    size = lib.g1_opt_workspace(n)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        rc = lib.g1_clip_grad_norm(n, _ptrs(grads), (ctypes.c_int * n)(*[_GRAD_TYPE[g.dtype] for g in grads]),
+                                   (ctypes.c_longlong * n)(*[g.numel() for g in grads]), float(max_norm), _dp(norm),
+                                   _dp(ws), size, _stream())
+    if rc:
+        _check()
+    torch.autograd.graph.increment_version(grads)
+    return norm
+
+
+class ClipAdam:
+    """Adam with the clipping of the global gradient norm taken into its step (g1_clip_adam): one pass over
+    gradients, parameters and moments in place of clip_grad_norm_ followed by torch.optim.Adam.step.
+
+    params: fp32 CUDA tensors on one device.  max_norm: the clip threshold (inf: none).  weight_decay is
+    decoupled (p *= 1 - lr * weight_decay).  lr may be a one-element fp32 CUDA tensor, read by the kernel.
+    moments: (first, second), lists of fp32 tensors laid out like the parameters, to be used in place
+    (made, zero, by default); steps: steps taken before.  Each parameter counts its own steps on the
+    device; one without a gradient is left alone, its count too, as in torch.
+
+    step() reads each parameter's .grad, step(grads) a list of fp32 / bf16 / fp16 gradients (None: left alone).
+    It returns the norm before clipping as a CUDA scalar; the gradients keep their values.  Nothing
+    synchronises, and a step captured into a CUDA graph counts on at each replay."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, max_norm=float("inf"), weight_decay=0.0,
+                 moments=None, steps=0):
+        _require_gpu()
+        load_library()
+        self.params = list(params)
+        if not self.params:
+            raise G1Error("no parameters")
+        self.device = _cuda_list(self.params, "parameters", (torch.float32,))
+        self.lr, self.betas, self.eps = lr, (float(betas[0]), float(betas[1])), float(eps)
+        self.max_norm, self.weight_decay = float(max_norm), float(weight_decay)
+        like = lambda: [torch.zeros_like(p, requires_grad=False) for p in self.params]
+        self.exp_avg, self.exp_avg_sq = (list(x) for x in moments) if moments is not None else (like(), like())
+        for ms in (self.exp_avg, self.exp_avg_sq):
+            if len(ms) != len(self.params):
+                raise G1Error("moments must be one tensor a parameter")
+            _cuda_list(ms + self.params[:1], "moments", (torch.float32,))
+            for m, p in zip(ms, self.params):
+                if m.shape != p.shape or m.stride() != p.stride():
+                    raise G1Error("moments must be laid out like their parameters")
+        self.steps = torch.full((len(self.params),), int(steps), dtype=torch.int64, device=self.device)
+
+    def zero_grad(self, set_to_none=True):
+        for p in self.params:
+            if set_to_none:
+                p.grad = None
+            elif p.grad is not None:
+                p.grad.zero_()
+
+    @torch.no_grad()
+    def step(self, grads=None):
+        params, n = self.params, len(self.params)
+        grads = [p.grad for p in params] if grads is None else list(grads)
+        if len(grads) != n:
+            raise G1Error("step takes one gradient (or None) a parameter")
+        for i, (g, p) in enumerate(zip(grads, params)):
+            if g is None:
+                continue
+            if g.shape != p.shape:
+                raise G1Error("gradients must have their parameters' shapes")
+            if g.stride() != p.stride() and g.numel():
+                if not g.is_cuda:
+                    raise G1Error("gradients must be CUDA tensors")
+                grads[i] = torch.empty_like(p, dtype=g.dtype).copy_(g)
+        have = [g for g in grads if g is not None]
+        _cuda_list(have + params[:1], "gradients", _GRAD_TYPE)
+        lib, dev = _lib, self.device
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        size = lib.g1_opt_workspace(n)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        lr_dev = None
+        if isinstance(self.lr, torch.Tensor):
+            if not (self.lr.device == dev and self.lr.dtype == torch.float32 and self.lr.numel() == 1):
+                raise G1Error("a tensor lr must be one fp32 number on the parameters' device")
+            lr_dev = self.lr
+        gp = (ctypes.c_void_p * n)(*[None if g is None else g.data_ptr() for g in grads])
+        types = (ctypes.c_int * n)(*[0 if g is None else _GRAD_TYPE[g.dtype] for g in grads])
+        counts = (ctypes.c_longlong * n)(*[0 if g is None else g.numel() for g in grads])
+        with _on(dev):
+            rc = lib.g1_clip_adam(n, gp, types, _ptrs(params), _ptrs(self.exp_avg), _ptrs(self.exp_avg_sq), counts,
+                                  _dp(self.steps), self.max_norm, 0.0 if lr_dev is not None else float(self.lr),
+                                  _dp(lr_dev), self.betas[0], self.betas[1], self.eps, self.weight_decay, _dp(norm),
+                                  _dp(ws), size, _stream())
+        if rc:
+            _check()
+        torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None]
+                                               + self.exp_avg + self.exp_avg_sq + [self.steps])
+        return norm
+
+    def state_dict(self):
+        lr = self.lr.detach().clone() if isinstance(self.lr, torch.Tensor) else self.lr
+        return dict(lr=lr, betas=self.betas, eps=self.eps, max_norm=self.max_norm, weight_decay=self.weight_decay,
+                    exp_avg=[m.clone() for m in self.exp_avg], exp_avg_sq=[v.clone() for v in self.exp_avg_sq],
+                    steps=self.steps.clone())
+
+    @torch.no_grad()
+    def load_state_dict(self, d):
+        if [tuple(m.shape) for m in d["exp_avg"]] != [tuple(p.shape) for p in self.params]:
+            raise G1Error("the state's moments do not have the parameters' shapes")
+        if isinstance(self.lr, torch.Tensor):
+            self.lr.copy_(torch.as_tensor(d["lr"]).reshape(self.lr.shape))
+        else:
+            self.lr = float(d["lr"])
+        self.betas, self.eps = tuple(d["betas"]), d["eps"]
+        self.max_norm, self.weight_decay = d["max_norm"], d["weight_decay"]
+        for ours, theirs in ((self.exp_avg, d["exp_avg"]), (self.exp_avg_sq, d["exp_avg_sq"])):
+            for a, b in zip(ours, theirs):
+                a.copy_(b)
+        self.steps.copy_(d["steps"])
 
 
 # ---------------- running obs normalizer (the state of ppo.py:63-81) ----------------

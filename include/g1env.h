@@ -174,6 +174,25 @@ int g1_obs_prep(long long rows, int dim, const float* O, const float* fmean, con
 int g1_adv_normalize(long long n, float* adv, const double* adv_mom, void* stream);
 int g1_runnorm_update(int dim, float* mean, float* var, double count, const double* obs_mom, void* stream);
 
+/* extension: the end of the trainer's update (reference counterpart: clip_grad_norm_ and the Adam step of
+ * scripts/ppo_fused.py:77-78,121-140), asynchronous on `stream` on the current device, 0 on success.  The
+ * lists are HOST arrays of n DEVICE pointers / values, read during the call only: grads[i] holds counts[i] numbers of
+ * types[i] (0 fp32, 1 bf16, 2 fp16), one after another; p, m, v fp32.  Tensors of length 0 are skipped.  Tensors of
+ * one call may not share memory.
+ *   norm (fp32 [1], DEVICE) <- sqrt(sum of all squares), summed in fp64; c = min(1, max_norm / (norm + 1e-6));
+ *   a norm that is NaN or infinite goes through that formula as it does in torch
+ *   g1_clip_grad_norm  grads *= c in place
+ *   g1_clip_adam       one Adam step (decoupled weight decay) of p with the gradients times c, which stay as they
+ *                      were; steps (DEVICE int64 [n]) counts each tensor's steps and is advanced by the call, so a
+ *                      captured call counts on; lr_dev (DEVICE fp32 [1] or NULL) takes the place of lr
+ * ws: DEVICE workspace of g1_opt_workspace(n) bytes, 16-byte aligned, for this call alone until it has run. */
+long long g1_opt_workspace(int n);
+int g1_clip_grad_norm(int n, void* const* grads, const int* types, const long long* counts, double max_norm, float* norm,
+                      void* ws, long long ws_size, void* stream);
+int g1_clip_adam(int n, void* const* grads, const int* types, float* const* p, float* const* m, float* const* v,
+                 const long long* counts, long long* steps, double max_norm, double lr, const float* lr_dev, double beta1,
+                 double beta2, double eps, double weight_decay, float* norm, void* ws, long long ws_size, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
