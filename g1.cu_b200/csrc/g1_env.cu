@@ -1869,3 +1869,4 @@ void g1_occupancy_report(void) {
 // trainer batch preparation (GAE, observation renormalisation, RunNorm update)
 #include "g1_ppo_prep.cuh"
 #include "g1_opt.cuh"
+#include "g1_gated.cuh"

@@ -60,6 +60,11 @@ SIGNATURES = {
     "g1_obs_prep": (ctypes.c_int, [ctypes.c_longlong, ctypes.c_int] + [_vp] * 6),
     "g1_adv_normalize": (ctypes.c_int, [ctypes.c_longlong, _vp, _vp, _vp]),
     "g1_runnorm_update": (ctypes.c_int, [ctypes.c_int, _vp, _vp, ctypes.c_double, _vp, _vp]),
+    "g1_gated_ff_workspace": (ctypes.c_longlong, [ctypes.c_int] * 3 + [_vp, ctypes.c_longlong, _vp, ctypes.c_int]),
+    "g1_gated_ff": (ctypes.c_int, [ctypes.c_int] * 5 + [_vp, ctypes.c_longlong] + [_vp] * 4 + [ctypes.c_longlong, _vp]),
+    "g1_gated_ff_backward": (ctypes.c_int, [ctypes.c_int] * 5 + [_vp, _vp, ctypes.c_longlong] + [_vp] * 4
+                             + [ctypes.c_int, _vp, _vp, ctypes.c_longlong, _vp]),
+    "g1_gated_ff_status": (ctypes.c_int, []),
     "g1_opt_workspace": (ctypes.c_longlong, [ctypes.c_int]),
     "g1_clip_grad_norm": (ctypes.c_int, [ctypes.c_int, _vp, _vp, _vp, ctypes.c_double, _vp, _vp, ctypes.c_longlong, _vp]),
     "g1_clip_adam": (ctypes.c_int, [ctypes.c_int] + [_vp] * 7 + [ctypes.c_double, ctypes.c_double, _vp]
@@ -281,6 +286,136 @@ def dense_bf16x3(X, W, bias=None, act=-1):
     return out
 
 
+# ---------------- gated layers ----------------
+_ACT = {"tanh": 0, "elu": 1, "silu": 2, "gelu": 3}
+_FF_TYPE = {torch.bfloat16: 1, torch.float16: 2}
+
+
+def _on(dev):
+    """Makes `dev` the current device for the calls within."""
+    return torch.cuda.device(dev)
+
+
+def _ff_args(x, w, b, act):
+    """Checked operands of a gated layer: rows [M, K] of x, w [2F, K] in x's type, b [2F] fp32 or None, act code."""
+    if not (x.is_cuda and w.is_cuda and (b is None or b.is_cuda)):
+        raise G1Error("a gated layer takes CUDA tensors (no CPU fallback)")
+    if x.dtype not in _FF_TYPE:
+        raise G1Error(f"a gated layer takes bf16 or fp16 rows, not {str(x.dtype)[6:]}")
+    if w.dtype != x.dtype:
+        raise G1Error("the weights must be of the rows' type")
+    if act not in _ACT:
+        raise G1Error(f"unknown activation {act!r} (one of {', '.join(_ACT)})")
+    if w.dim() != 2 or w.shape[0] % 2 or not w.numel() or x.dim() < 1 or x.shape[-1] != w.shape[1]:
+        raise G1Error("a gated layer takes x [..., K] and w [2F, K]")
+    if b is not None and (b.shape != w.shape[:1] or not b.is_floating_point()):
+        raise G1Error("the bias must be [2F]")
+    if w.device != x.device or (b is not None and b.device != x.device):
+        raise G1Error("a gated layer's tensors must be on one device")
+    x2 = x.reshape(-1, x.shape[-1])
+    if x2.stride(1) != 1 and x2.shape[1] > 1 or x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]:
+        x2 = x2.contiguous()
+    if x2.shape[0] > 1 << 30:
+        raise G1Error("too many rows")
+    return x2, w.contiguous(), None if b is None else b.float().contiguous(), _ACT[act]
+
+
+def _ff_ws(lib, x2, w, F, backward):
+    """(rows, K, ld) and the workspace of a call; None where it needs none."""
+    M, K = x2.shape
+    ld = x2.stride(0) if M > 1 else K
+    n = lib.g1_gated_ff_workspace(M, K, F, _dp(x2), ld, _dp(w), backward)
+    return M, K, ld, n, torch.empty(n, dtype=torch.uint8, device=x2.device) if n else None
+
+
+def gated_ff_device(x, w, b=None, act="silu"):
+    """One gated layer, h = act(x Wg^T + bg) * (x Wu^T + bu) (g1_gated_ff): x [..., K] bf16 or fp16, w [2F, K] of the
+    same type (the F gate rows, then the F up rows), b [2F] or None, act "tanh", "elu", "silu" or "gelu" (erf).
+    Returns h [..., F] in x's type, on torch's current stream.  Rows may be strided; rows or weights that do
+    not start on 16-byte boundaries (K not a multiple of 8) are copied first."""
+    lib = load_library()
+    x2, w, b, code = _ff_args(x, w, b, act)
+    F = w.shape[0] // 2
+    with _on(x.device):
+        M, K, ld, n, ws = _ff_ws(lib, x2, w, F, 0)
+        h = torch.empty(x.shape[:-1] + (F,), dtype=x.dtype, device=x.device)
+        if lib.g1_gated_ff(M, K, F, _FF_TYPE[x.dtype], code, _dp(x2), ld, _dp(w), _dp(b), _dp(h), _dp(ws), n, _stream()):
+            _check()
+    return h
+
+
+def gated_ff_backward_device(dh, x, w, b=None, act="silu", need=(True, True, True), dw_dtype=None):
+    """The gradients of gated_ff_device for dh [..., F] (g1_gated_ff_backward): dx like x, dw [2F, K] (dw_dtype: x's type
+    or fp32), db [2F] fp32; None where `need` (dx, dw, db) says so.  Nothing of the forward pass but its inputs
+    is needed.  dg and du are rounded to x's type before the products with W and x, but not in db."""
+    lib = load_library()
+    x2, w, b, code = _ff_args(x, w, b, act)
+    F = w.shape[0] // 2
+    dw_dtype = x.dtype if dw_dtype is None else dw_dtype
+    if dw_dtype not in (x.dtype, torch.float32):
+        raise G1Error("dw is fp32 or of the rows' type")
+    if dh.device != x.device or dh.dtype != x.dtype or tuple(dh.shape) != tuple(x.shape[:-1]) + (F,):
+        raise G1Error("dh must be [..., F] on x's device and of its type")
+    dh = dh.contiguous()
+    dev = x.device
+    with _on(dev):
+        M, K, ld, n, ws = _ff_ws(lib, x2, w, F, 1)
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
+        dw = torch.empty(2 * F, K, dtype=dw_dtype, device=dev) if need[1] else None
+        db = torch.empty(2 * F, dtype=torch.float32, device=dev) if need[2] else None
+        if lib.g1_gated_ff_backward(M, K, F, _FF_TYPE[x.dtype], code, _dp(dh), _dp(x2), ld, _dp(w), _dp(b), _dp(dx),
+                                    _dp(dw), _FF_TYPE.get(dw_dtype, 0), _dp(db), _dp(ws), n, _stream()):
+            _check()
+    return dx, dw, db
+
+
+def gated_ff_status():
+    """Nonzero if a wait inside a gated layer's kernels ran out since the last call (synchronous; clears)."""
+    return load_library().g1_gated_ff_status()
+
+
+class _GatedFF(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b, act):
+        w16 = w if w.dtype == x.dtype else w.to(x.dtype)
+        ctx.save_for_backward(x, w16, b)
+        ctx.act, ctx.w_dtype = act, w.dtype
+        return gated_ff_device(x, w16, b, act)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        x, w16, b = ctx.saved_tensors
+        need = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], b is not None and ctx.needs_input_grad[2])
+        dx, dw, db = gated_ff_backward_device(dh, x, w16, b, ctx.act, need, ctx.w_dtype)
+        return dx, dw, db if db is None else db.to(b.dtype), None
+
+
+def gated_ff(x, w, b=None, act="silu"):
+    """gated_ff_device with gradients.  w may be fp32 beside 16-bit rows: it is rounded to their type for the
+    products, and its gradient comes back in fp32.  The forward pass keeps only its inputs."""
+    if w.dtype not in (x.dtype, torch.float32):
+        raise G1Error("the weights must be fp32 or of the rows' type")
+    return _GatedFF.apply(x, w, b, act)
+
+
+class GatedLinear(nn.Module):
+    """A gated layer with fp32 parameters, weight [2F, K] (gate rows, then up rows) and bias [2F], on rows that are taken
+    to `dtype`.  Initialised as nn.Linear(K, 2F)."""
+
+    def __init__(self, in_features, out_features, act="silu", bias=True, dtype=torch.bfloat16):
+        super().__init__()
+        lin = nn.Linear(in_features, 2 * out_features, bias=bias)
+        self.weight, self.bias = lin.weight, lin.bias
+        self.in_features, self.out_features, self.act, self.dtype = in_features, out_features, act, dtype
+
+    def forward(self, x):
+        return gated_ff(x.to(self.dtype), self.weight, self.bias, self.act)
+
+    def extra_repr(self):
+        return f"{self.in_features}, {self.out_features}, act={self.act}"
+
+
 # ---------------- trainer batch preparation (ppo_fused.py:104-119, ppo.py:71-79) ----------------
 def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
@@ -338,11 +473,6 @@ def runnorm_update_device(norm, obs_mom, rows_total):
 
 # ---------------- gradient norm, clipping and the clipped Adam step ----------------
 _GRAD_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
-
-def _on(dev):
-    """Makes `dev` the current device for the calls within (nothing where it is already)."""
-    return torch.cuda.device(dev)
 
 
 def _dense(t):

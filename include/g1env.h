@@ -174,6 +174,26 @@ int g1_obs_prep(long long rows, int dim, const float* O, const float* fmean, con
 int g1_adv_normalize(long long n, float* adv, const double* adv_mom, void* stream);
 int g1_runnorm_update(int dim, float* mean, float* var, double count, const double* obs_mom, void* stream);
 
+/* extension: one gated policy layer on the tensor cores (tcgen05), beside g1_gemm_bf16_tc's plain one:
+ *     h = act(X Wg^T + bg) * (X Wu^T + bu)
+ * X [M][K] (row stride ldx), W [2F][K] = [Wg; Wu] row-major, b fp32 [2F] = [bg; bu] or NULL, h [M][F]; X, W, h of one
+ * type: 1 bf16, 2 fp16; fp32 sums, one rounding at the end; act 0 tanh, 1 ELU, 2 SiLU, 3 GELU (erf).  DEVICE
+ * pointers on the current device, asynchronous on `stream`, 0 on success.
+ *   g1_gated_ff_backward  from dh [M][F]: dx [M][K], dw [2F][K] (dw_type 0 fp32, or the inputs' type), db fp32
+ *                         [2F]; any of the three may be NULL.  g and u are computed again from X; dg and du are rounded
+ *                         to the inputs' type before their products (not in db).  Same inputs, same bits.
+ * ws: DEVICE workspace of g1_gated_ff_workspace(...) bytes, 256-byte aligned, for this call alone until it has run (it
+ * also holds copies of X and W where their rows do not start on 16-byte boundaries).
+ *   g1_gated_ff_status    nonzero if a wait of these kernels ran out on the current device since the last call
+ *                         (synchronous; clears) */
+long long g1_gated_ff_workspace(int M, int K, int F, const void* X, long long ldx, const void* W, int backward);
+int g1_gated_ff(int M, int K, int F, int type, int act, const void* X, long long ldx, const void* W, const float* b, void* h,
+                void* ws, long long ws_size, void* stream);
+int g1_gated_ff_backward(int M, int K, int F, int type, int act, const void* dh, const void* X, long long ldx, const void* W,
+                         const float* b, void* dx, void* dw, int dw_type, float* db, void* ws, long long ws_size,
+                         void* stream);
+int g1_gated_ff_status(void);
+
 /* extension: the end of the trainer's update (reference counterpart: clip_grad_norm_ and the Adam step of
  * scripts/ppo_fused.py:77-78,121-140), asynchronous on `stream` on the current device, 0 on success.  The
  * lists are HOST arrays of n DEVICE pointers / values, read during the call only: grads[i] holds counts[i] numbers of
