@@ -36,8 +36,22 @@ namespace g1ff {
 using g1gemm::s32;
 using g1gemm::tma_load_2d;
 
-constexpr int BM = 128, BK = 64, STAGES = 4, EPI_WARPS = 16, NTH = 64 + 32 * EPI_WARPS;
+constexpr int BM = 128, BK = 64;  // rows of A a CTA, chunk of the sum
 enum { FWD = 0, DZ = 1, DX = 2, DW = 3 };
+// CG: CTAs that work on a tile together (cta_group); BN: columns of B a tile
+template <int MODE, int BN, int CG>
+struct Cfg {
+    static constexpr bool PAIR = MODE == FWD || MODE == DZ;
+    static constexpr int TN = PAIR ? BN / 2 : BN;                  // output columns a tile
+    static constexpr int PARTS = TN >= 64 ? 4 : TN / 16;           // epilogue warps a TMEM lane quarter
+    static constexpr int EPI = 4 * PARTS, NTH = 64 + 32 * EPI;
+    static constexpr int CW = TN / PARTS, SC = CW >= 32 ? 32 : 16; // columns a warp, and a step of it
+    static constexpr int LD = SC + 8;                              // 16-bit numbers a row of a warp's buffer (no bank conflicts)
+    static constexpr int NB = BN / CG;                             // columns of B in this CTA's memory
+    static constexpr int STAGES = MODE == DZ ? 4 : MODE == DW ? 6 : 5;
+    static constexpr int BUFS = MODE == DZ ? 2 : MODE == DW ? 0 : 1;
+    static constexpr int STAGE_BYTES = (BM + NB) * BK * 2;
+};
 constexpr int DW_BLOCK = 64;  // chunks (of 64 rows) that the CTAs of DW walk together
 
 __device__ int g_err;  // a wait ran out
@@ -52,7 +66,7 @@ struct Args {
     long long ldo;
     float* db;                   // DZ: [gridDim][4][2F] column sums, zeroed, or null
     int tile0, ntp;              // DW: the pass's tiles
-    int vec;                     // rows of the output (and of dh) are 16-byte aligned
+    int vec;                     // rows of the output and of dh are 16-byte aligned
 };
 
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
@@ -141,59 +155,68 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
         : "r"(taddr));
 }
 
-template <int BN>
+// A launch may start while the one before it in the stream ends (programmatic dependent launch): set up, then wait here
+// before the first access to memory that another kernel writes.
+__device__ __forceinline__ void after_previous() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+}
+
+template <int MODE, int BN, int CG>
 struct Smem {
-    uint8_t a[STAGES][BM * BK * 2];
-    uint8_t b[STAGES][BN * BK * 2];
-    uint64_t full[STAGES], empty[STAGES], tfull[2], tempty[2];
+    using C = Cfg<MODE, BN, CG>;
+    uint8_t a[C::STAGES][BM * BK * 2];
+    uint8_t b[C::STAGES][C::NB * BK * 2];
+    uint8_t buf[C::BUFS ? C::EPI : 1][C::BUFS ? C::BUFS : 1][C::BUFS ? 32 * C::LD * 2 : 16];
+    float bias[C::PAIR ? C::EPI : 1][2][32];
+    uint64_t full[C::STAGES], empty[C::STAGES], tfull[2], tempty[2];
     uint32_t tslot;
     volatile int stop;  // a wait of this CTA ran out
 };
-template <int BN>
-constexpr int smem_bytes() { return (int)sizeof(Smem<BN>) + 1024; }
+template <int MODE, int BN, int CG>
+constexpr int smem_bytes() { return (int)sizeof(Smem<MODE, BN, CG>) + 1024; }
 
-// 16 values of a row to 16-bit memory, `n` of them inside the matrix
-template <class T>
-__device__ __forceinline__ void store16(T* dst, const float* v, int n, bool vec) {
-    if (vec && n >= 16) {
-        uint32_t pk[8];
+// A warp's 32 rows x SC columns go to and from global memory through its buffer, so that neighbouring lanes touch
+// neighbouring addresses: one row a lane would touch 32 lines with each access (measured on DZ, 524288 x 1024 x 512:
+// REPLACE_ME us that way).  vec: rows on 16-byte boundaries.
+template <class T, int SC, int LD>
+__device__ __forceinline__ void rows_out(const uint8_t* buf, T* m, long long ld, int row0, int M, int col, int N, bool vec,
+                                         int lane) {
+    if (vec) {
+        constexpr int CH = SC / 8;
+        const int ch = lane % CH;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) pk[j] = Half2<T>::pack(v[2 * j], v[2 * j + 1]);
-        reinterpret_cast<uint4*>(dst)[0] = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-        reinterpret_cast<uint4*>(dst)[1] = make_uint4(pk[4], pk[5], pk[6], pk[7]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-            if (j < n) dst[j] = Half2<T>::one(v[j]);
-    }
-}
-
-__device__ __forceinline__ void load_bias(const float* bias, int n, float* v) {
-#pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] = (bias && j < n) ? __ldg(bias + j) : 0.f;
-}
-
-template <class T>
-__device__ __forceinline__ void load16(const T* src, float* v, int n, bool vec) {
-    if (vec && n >= 16) {
-        const uint4 a = __ldcs(reinterpret_cast<const uint4*>(src)), b = __ldcs(reinterpret_cast<const uint4*>(src) + 1);
-        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float2 f = Half2<T>::unpack(w[j]);
-            v[2 * j] = f.x;
-            v[2 * j + 1] = f.y;
+        for (int i = 0; i < CH; ++i) {
+            const int r = lane / CH + i * (32 / CH);
+            if (row0 + r < M && col + 8 * ch < N)
+                *reinterpret_cast<uint4*>(m + (size_t)(row0 + r) * ld + col + 8 * ch) =
+                    *reinterpret_cast<const uint4*>(buf + r * LD * 2 + ch * 16);
         }
     } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = j < n ? Half2<T>::f(src[j]) : 0.f;
+        const int c = lane % SC;
+#pragma unroll 8
+        for (int i = 0; i < SC; ++i) {
+            const int r = lane / SC + i * (32 / SC);
+            if (row0 + r < M && col + c < N)
+                m[(size_t)(row0 + r) * ld + col + c] = reinterpret_cast<const T*>(buf)[r * LD + c];
+        }
+    }
+}
+template <class T, int SC, int LD>
+__device__ __forceinline__ void rows_in_any(uint8_t* buf, const T* m, long long ld, int row0, int M, int col, int N, int lane) {
+    const int c = lane % SC;
+#pragma unroll 8
+    for (int i = 0; i < SC; ++i) {
+        const int r = lane / SC + i * (32 / SC);
+        reinterpret_cast<T*>(buf)[r * LD + c] =
+            row0 + r < M && col + c < N ? m[(size_t)(row0 + r) * ld + col + c] : Half2<T>::one(0.f);
     }
 }
 
-// lane l gets the sum over the warp's lanes of v[l]: halves of the list change sides 5 times (31 shuffles)
-__device__ __forceinline__ float column_sums(float (&v)[32], int lane) {
+// lane l gets the sum over the warp's lanes of v[l % 16]: halves of the list change sides 4 times
+__device__ __forceinline__ float column_sums(float (&v)[16], int lane) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+    for (int o = 8; o > 0; o >>= 1) {
         const bool up = lane & o;
 #pragma unroll
         for (int j = 0; j < o; ++j) {
@@ -201,31 +224,99 @@ __device__ __forceinline__ float column_sums(float (&v)[32], int lane) {
             v[j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
         }
     }
-    return v[0];
+    return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 16);
 }
 
-template <class T, int ACT>
-__device__ __forceinline__ void fwd16(const uint32_t* rg, const uint32_t* ru, const float* bg, const float* bu, float* h) {
+// h of 8 columns
+template <int ACT>
+__device__ __forceinline__ void fwd8(const uint32_t* rg, const uint32_t* ru, const float* bg, const float* bu, float* h) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
+    for (int j = 0; j < 8; ++j) {
         float a, d;
         act1<ACT, false>(__uint_as_float(rg[j]) + bg[j], a, d);
         h[j] = a * (__uint_as_float(ru[j]) + bu[j]);
     }
 }
+// z of 8 columns: dg, du.  dh is packed 16-bit pairs
 template <class T, int ACT>
-__device__ __forceinline__ void dz16(const uint32_t* rg, const uint32_t* ru, const float* bg, const float* bu,
-                                     const float* dh, float* z) {
+__device__ __forceinline__ void dz8(const uint32_t* rg, const uint32_t* ru, const float* bg, const float* bu, uint4 dh4,
+                                    float* z) {
+    const uint32_t w[4] = {dh4.x, dh4.y, dh4.z, dh4.w};
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
+    for (int j = 0; j < 8; ++j) {
+        const float2 p = Half2<T>::unpack(w[j / 2]);
+        const float dh = j & 1 ? p.y : p.x;
         float a, d;
         act1<ACT, true>(__uint_as_float(rg[j]) + bg[j], a, d);
-        z[j] = dh[j] * (__uint_as_float(ru[j]) + bu[j]) * d;
-        z[16 + j] = dh[j] * a;
+        z[j] = dh * (__uint_as_float(ru[j]) + bu[j]) * d;
+        z[8 + j] = dh * a;
     }
 }
+template <class T>
+__device__ __forceinline__ uint4 pack8(const float* v) {
+    return make_uint4(Half2<T>::pack(v[0], v[1]), Half2<T>::pack(v[2], v[3]), Half2<T>::pack(v[4], v[5]),
+                      Half2<T>::pack(v[6], v[7]));
+}
 
-// The tiles of a CTA.  FWD, DZ, DX: 128-row blocks by column tiles, columns fastest, so that the CTAs in flight
+// ---- two CTAs on a tile
+__device__ __forceinline__ uint32_t cta_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t at_leader(uint32_t saddr) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(saddr));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+// a load into this CTA's memory; its bytes count at `bar`, which may lie in the tile's first CTA
+template <int CG>
+__device__ __forceinline__ void load2d(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    if constexpr (CG == 1)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+                s32(dst)),
+            "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], "
+            "[%4];" ::"r"(s32(dst)),
+            "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void mma16(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accum) {
+    if constexpr (CG == 1)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(ad), "l"(bd), "r"(idesc), "r"(accum));
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+            "l"(ad), "l"(bd), "r"(idesc), "r"(accum));
+}
+// arrives on the barrier at this offset in every CTA of the tile once the MMAs issued so far are done
+template <int CG>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    if constexpr (CG == 1)
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(s32(bar)) : "memory");
+    else
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(s32(bar)),
+            "h"((uint16_t)3)
+            : "memory");
+}
+
+// The tiles of a CTA (of a group of CG).  FWD, DZ, DX: row blocks by column tiles, columns fastest, so that the CTAs in flight
 // share rows of A in L2 and A comes from HBM once (the weights stay in L2).
 // DW: the sum over M is cut for the CTAs to be equally loaded, each CTA keeping at most two tiles (two
 // accumulators) from start to end: rows are walked in blocks of DW_BLOCK chunks, and of each block's ntp x DW_BLOCK
@@ -235,35 +326,42 @@ template <int MODE>
 struct Tiles {
     int tile, step, count, acc;      // FWD, DZ, DX
     int t0, c0, c1, c2, blk;         // DW: chunks [c0, c1) of tile t0 and [0, c2) of tile t0 + 1 in each block
-    __device__ __forceinline__ Tiles(const Args& P, int ntiles) {
+    // id-th of n CTAs (or groups of CTAs)
+    __device__ __forceinline__ Tiles(const Args& P, int ntiles, int id, int n) {
         if (MODE == DW) {
             blk = min(DW_BLOCK, P.nk);
             const long long U = (long long)P.ntp * blk;
-            const long long u0 = U * blockIdx.x / gridDim.x, u1 = U * (blockIdx.x + 1) / gridDim.x;
+            const long long u0 = U * id / n, u1 = U * (id + 1) / n;
             t0 = (int)(u0 / blk);
             c0 = (int)(u0 % blk);
             c1 = (int)min((long long)blk, c0 + (u1 - u0));
             c2 = (int)(u1 - u0) - (c1 - c0);
         } else {
-            tile = blockIdx.x;
-            step = gridDim.x;
+            tile = id;
+            step = n;
             count = ntiles;
         }
     }
 };
 
-template <class T, int MODE, int BN>
-__global__ void __launch_bounds__(NTH, 1) k_ff(const __grid_constant__ Args P) {
+template <class T, int MODE, int BN, int CG>
+__global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid_constant__ Args P) {
+    using C = Cfg<MODE, BN, CG>;
     extern __shared__ uint8_t smem_raw[];
-    Smem<BN>& S = *reinterpret_cast<Smem<BN>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    constexpr bool A_MN = MODE == DW, B_MN = MODE == DX || MODE == DW, PAIR = MODE == FWD || MODE == DZ;
-    constexpr int TN = PAIR ? BN / 2 : BN;  // output columns a tile
+    auto& S = *reinterpret_cast<Smem<MODE, BN, CG>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    constexpr bool A_MN = MODE == DW, B_MN = MODE == DX || MODE == DW, PAIR = C::PAIR;
+    constexpr int TN = C::TN, STAGES = C::STAGES, NB = C::NB;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = CG == 1 ? 0 : (int)cta_rank();
     const int ntn = (P.N + TN - 1) / TN;
-    // DW: row tiles of the gate half, then of the up half
+    // DW: 128-row tiles of the gate half, then of the up half
     const int half_tiles = (P.F + BM - 1) / BM;
-    const int ntm = MODE == DW ? 2 * half_tiles : (P.M + BM - 1) / BM;
+    const int ntm = MODE == DW ? 2 * half_tiles / CG : (P.M + BM * CG - 1) / (BM * CG);
     const int ntiles = ntm * ntn, nk = P.nk;
+    if (tid == 32) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&P.a0) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&P.b0) : "memory");
+    }
     if (tid == 0) {
         S.stop = 0;
         for (int i = 0; i < STAGES; ++i) {
@@ -272,49 +370,64 @@ __global__ void __launch_bounds__(NTH, 1) k_ff(const __grid_constant__ Args P) {
         }
         for (int i = 0; i < 2; ++i) {
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(s32(&S.tfull[i])));
-            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(s32(&S.tempty[i])), "r"(EPI_WARPS));
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(s32(&S.tempty[i])), "r"(CG * C::EPI));
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&S.tslot)), "r"(2 * BN));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        __syncwarp();
+        if constexpr (CG == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&S.tslot)), "r"(2 * BN));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s32(&S.tslot)), "r"(2 * BN));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;");
     __syncthreads();
+    if (CG > 1) cluster_sync();  // the other CTA's barriers are ready
     asm volatile("tcgen05.fence::after_thread_sync;");
     const uint32_t tmem = S.tslot;
     bool ok = true;
-    const Tiles<MODE> W(P, ntiles);
+    after_previous();
+    const Tiles<MODE> W(P, ntiles, blockIdx.x / CG, gridDim.x / CG);
 
-    if (warp == 0 && lane == 0) {  // loads
+    if (warp == 0 && lane == 0) {  // loads: this CTA's rows of A and its share of B
         int stage = 0;
         uint32_t phase = 0;
         auto load = [&](int tile, int c) -> bool {
             if (!wait(&S.empty[stage], phase ^ 1u)) return false;
-            uint64_t* bar = &S.full[stage];
-            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(s32(bar)), "r"((BM + BN) * BK * 2)
-                         : "memory");
-            const int mt = tile / ntn, n0 = (tile % ntn) * TN;
+            uint32_t bar = s32(&S.full[stage]);
+            if (rank == 0)
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(CG * C::STAGE_BYTES)
+                             : "memory");
+            if (CG > 1) bar = at_leader(bar);
+            const int mt = (tile / ntn) * CG + rank, n0 = (tile % ntn) * TN;
             uint8_t *as = S.a[stage], *bs = S.b[stage];
             if (PAIR) {
-                tma_load_2d(as, &P.a0, c * BK, mt * BM, bar);
-                tma_load_2d(bs, &P.b0, c * BK, n0, bar);
-                tma_load_2d(bs + TN * BK * 2, &P.b1, c * BK, n0, bar);
+                load2d<CG>(as, &P.a0, c * BK, mt * BM, bar);
+                if (CG == 1) {
+                    load2d<CG>(bs, &P.b0, c * BK, n0, bar);
+                    load2d<CG>(bs + TN * BK * 2, &P.b1, c * BK, n0, bar);
+                } else {
+                    load2d<CG>(bs, rank == 0 ? &P.b0 : &P.b1, c * BK, n0, bar);
+                }
             } else if (MODE == DX) {
                 // the sum runs over the gate half's columns, then the up half's
                 const bool up = c >= nk / 2;
                 const int k0 = (up ? c - nk / 2 : c) * BK;
-                tma_load_2d(as, up ? &P.a1 : &P.a0, k0, mt * BM, bar);
+                load2d<CG>(as, up ? &P.a1 : &P.a0, k0, mt * BM, bar);
 #pragma unroll
-                for (int j = 0; j < BN / 64; ++j) tma_load_2d(bs + j * 8192, up ? &P.b1 : &P.b0, n0 + 64 * j, k0, bar);
+                for (int j = 0; j < NB / 64; ++j)
+                    load2d<CG>(bs + j * 8192, up ? &P.b1 : &P.b0, n0 + rank * NB + 64 * j, k0, bar);
             } else {
                 const bool up = mt >= half_tiles;
                 const int f0 = (up ? mt - half_tiles : mt) * BM;
 #pragma unroll
-                for (int j = 0; j < BM / 64; ++j) tma_load_2d(as + j * 8192, up ? &P.a1 : &P.a0, f0 + 64 * j, c * BK, bar);
+                for (int j = 0; j < BM / 64; ++j) load2d<CG>(as + j * 8192, up ? &P.a1 : &P.a0, f0 + 64 * j, c * BK, bar);
 #pragma unroll
-                for (int j = 0; j < BN / 64; ++j) tma_load_2d(bs + j * 8192, &P.b0, n0 + 64 * j, c * BK, bar);
+                for (int j = 0; j < NB / 64; ++j) load2d<CG>(bs + j * 8192, &P.b0, n0 + rank * NB + 64 * j, c * BK, bar);
             }
             if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             return true;
@@ -330,9 +443,10 @@ __global__ void __launch_bounds__(NTH, 1) k_ff(const __grid_constant__ Args P) {
             for (int tile = W.tile; tile < ntiles && ok; tile += W.step)
                 for (int c = 0; c < nk && ok; ++c) ok = load(tile, c);
         }
-    } else if (warp == 1 && lane == 0) {  // MMAs
+        // every load of this CTA has landed before it leaves: the first CTA's MMA thread has seen them all, or gave up
+    } else if (warp == 1 && lane == 0 && rank == 0) {  // MMAs, of both CTAs
         constexpr uint32_t idesc = (1u << 4) | (Half2<T>::fmt << 7) | (Half2<T>::fmt << 10) | ((A_MN ? 1u : 0u) << 15) |
-                                   ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+                                   ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(CG * BM >> 4) << 24);
         int stage = 0;
         uint32_t phase = 0;
         auto mma = [&](uint32_t d, bool first) -> bool {
@@ -343,23 +457,11 @@ __global__ void __launch_bounds__(NTH, 1) k_ff(const __grid_constant__ Args P) {
             for (int k = 0; k < BK / 16; ++k) {
                 const uint64_t ad = A_MN ? desc_mn(a0 + k * 2048) : g1gemm::desc_sw128(a0 + k * 32);
                 const uint64_t bd = B_MN ? desc_mn(b0 + k * 2048) : g1gemm::desc_sw128(b0 + k * 32);
-                const uint32_t accum = (!first || k > 0) ? 1u : 0u;
-                asm volatile(
-                    "{\n\t.reg .pred p;\n\t"
-                    "setp.ne.b32 p, %4, 0;\n\t"
-                    "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-                    "l"(ad), "l"(bd), "r"(idesc), "r"(accum));
+                mma16<CG>(d, ad, bd, idesc, (!first || k > 0) ? 1u : 0u);
             }
-            asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                             s32(&S.empty[stage]))
-                         : "memory");
+            commit<CG>(&S.empty[stage]);
             if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             return true;
-        };
-        auto commit = [&](int acc) {
-            asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                             s32(&S.tfull[acc]))
-                         : "memory");
         };
         if (MODE == DW) {
             for (int base = 0; base < nk && ok; base += W.blk) {
@@ -368,24 +470,23 @@ __global__ void __launch_bounds__(NTH, 1) k_ff(const __grid_constant__ Args P) {
                 for (int c = 0; c < W.c2 && ok; ++c)
                     if (base + c < nk) ok = mma(tmem + BN, base == 0 && c == 0);
             }
-            if (ok) { commit(0); commit(1); }
+            if (ok) { commit<CG>(&S.tfull[0]); commit<CG>(&S.tfull[1]); }
         } else {
             uint32_t acc = 0, accph = 0;
             for (int tile = W.tile; tile < ntiles && ok; tile += W.step) {
                 if (!wait(&S.tempty[acc], accph ^ 1u)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;");
                 for (int c = 0; c < nk && ok; ++c) ok = mma(tmem + acc * BN, c == 0);
-                if (ok) commit(acc);
+                if (ok) commit<CG>(&S.tfull[acc]);
                 if (++acc == 2) { acc = 0; accph ^= 1u; }
             }
         }
     } else if (warp >= 2) {  // epilogue: warp w reads TMEM lanes 32 (w & 3) .., part (w - 2) / 4 of the columns
         const int q = warp & 3, part = (warp - 2) >> 2;
-        constexpr int CW = TN / 4;
-        static_assert(CW % 16 == 0, "16-column TMEM loads");
+        constexpr int CW = C::CW, SC = C::SC, LD = C::LD;
         const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16);
         if (MODE == DW) {
-            // fp32 partial tiles, row-major [128][BN]; slot b + t is this CTA's alone (a next share raises b or t)
+            // fp32 partial tiles, row-major; slot (group + tile) is this group's alone (the next share raises one of them)
             for (int a = 0; a < 2 && ok; ++a) {
                 const bool have = a == 0 ? W.c1 > W.c0 : W.c2 > 0;
                 if (!have) continue;
@@ -394,7 +495,8 @@ __global__ void __launch_bounds__(NTH, 1) k_ff(const __grid_constant__ Args P) {
                 for (int i = 0; i < 64 && !ok && !S.stop; ++i) ok = wait(&S.tfull[a], 0);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;");
-                float* dst = (float*)P.out + ((size_t)(blockIdx.x + W.t0 + a) * BM + 32 * q + lane) * BN + part * CW;
+                const size_t row = ((size_t)(blockIdx.x / CG + W.t0 + a) * CG + rank) * BM + 32 * q + lane;
+                float* dst = (float*)P.out + row * BN + part * CW;
 #pragma unroll 1
                 for (int cc = 0; cc < CW; cc += 16) {
                     uint32_t r[16];
@@ -407,69 +509,127 @@ __global__ void __launch_bounds__(NTH, 1) k_ff(const __grid_constant__ Args P) {
             }
         } else {
             uint32_t acc = 0, accph = 0;
+            uint8_t* buf = S.buf[warp - 2][0];
+            uint8_t* buf2 = S.buf[warp - 2][C::BUFS - 1];
+            float(*sb)[32] = S.bias[PAIR ? warp - 2 : 0];
+            const uint32_t tempty0 = CG == 1 ? 0 : at_leader(s32(&S.tempty[0])), tempty1 = CG == 1 ? 0 : at_leader(s32(&S.tempty[1]));
+            // the bias (a column a lane) and dh (as rows_out lays out its accesses) of a step are asked for one step ahead,
+            // a tile's first before the wait for its products
+            constexpr int CH = SC / 8;
+            uint4 nx[CH];
+            float nbg = 0.f, nbu = 0.f;
+            auto ask = [&](int tile, int cc) {
+                if (!PAIR || tile >= ntiles) return;
+                const int col = (tile % ntn) * TN + part * CW + cc;
+                nbg = nbu = 0.f;
+                if (P.bias && lane < SC && col + lane < P.N) {
+                    nbg = __ldg(P.bias + col + lane);
+                    nbu = __ldg(P.bias + P.F + col + lane);
+                }
+                if (MODE == DZ && P.vec) {
+                    const int row0 = ((tile / ntn) * CG + rank) * BM + 32 * q, ch = lane % CH;
+#pragma unroll
+                    for (int i = 0; i < CH; ++i) {
+                        const int r = row0 + lane / CH + i * (32 / CH);
+                        nx[i] = r < P.M && col + 8 * ch < P.N
+                                    ? __ldcs(reinterpret_cast<const uint4*>((const T*)P.dh + (size_t)r * P.F + col + 8 * ch))
+                                    : make_uint4(0, 0, 0, 0);
+                    }
+                }
+            };
+            ask(W.tile, 0);
             for (int tile = W.tile; tile < ntiles; tile += W.step) {
                 if (!wait(&S.tfull[acc], accph)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;");
-                const int row = (tile / ntn) * BM + 32 * q + lane, n0 = (tile % ntn) * TN + part * CW;
+                const int row0 = ((tile / ntn) * CG + rank) * BM + 32 * q, row = row0 + lane;
                 const uint32_t t0 = tl + acc * BN + part * CW;
 #pragma unroll 1
-                for (int cc = 0; cc < CW; cc += 16) {
-                    const int col = n0 + cc, left = P.N - col;
-                    if (left <= 0) break;  // the same for the whole warp
-                    uint32_t r[16];
-                    tmem_ld16(t0 + cc, r);
-                    if (PAIR) {
-                        uint32_t ru[16];
-                        tmem_ld16(t0 + TN + cc, ru);
-                        float bg[16], bu[16];
-                        load_bias(P.bias ? P.bias + col : nullptr, left, bg);
-                        load_bias(P.bias ? P.bias + P.F + col : nullptr, left, bu);
-                        if (MODE == FWD) {
-                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                            float h[16];
-                            if (P.act == 0) fwd16<T, 0>(r, ru, bg, bu, h);
-                            else if (P.act == 1) fwd16<T, 1>(r, ru, bg, bu, h);
-                            else if (P.act == 2) fwd16<T, 2>(r, ru, bg, bu, h);
-                            else fwd16<T, 3>(r, ru, bg, bu, h);
-                            if (row < P.M) store16((T*)P.out + (size_t)row * P.ldo + col, h, left, P.vec);
-                        } else {
-                            float dh[16], z[32];
-                            if (row < P.M) load16((const T*)P.dh + (size_t)row * P.F + col, dh, left, P.vec);
-                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                            if (P.act == 0) dz16<T, 0>(r, ru, bg, bu, dh, z);
-                            else if (P.act == 1) dz16<T, 1>(r, ru, bg, bu, dh, z);
-                            else if (P.act == 2) dz16<T, 2>(r, ru, bg, bu, dh, z);
-                            else dz16<T, 3>(r, ru, bg, bu, dh, z);
-                            if (row < P.M) {
-                                // z's rows are padded to whole 16-byte groups: always aligned
-                                T* dst = (T*)P.out + (size_t)row * P.ldo + col;
-                                store16(dst, z, left, true);
-                                store16(dst + P.ldo / 2, z + 16, left, true);
-                            }
-                            if (P.db) {
-                                if (row >= P.M) {  // rows behind the last one add nothing, whatever they hold
+                for (int cc = 0; cc < CW; cc += SC) {
+                    const int col = (tile % ntn) * TN + part * CW + cc;
+                    const bool some = col < P.N;  // the same for the whole warp
+                    if (some && PAIR) {
+                        if (lane < SC) { sb[0][lane] = nbg; sb[1][lane] = nbu; }
+                        if (MODE == DZ) {
+                            if (P.vec) {
 #pragma unroll
-                                    for (int j = 0; j < 32; ++j) z[j] = 0.f;
-                                }
-                                const float s = column_sums(z, lane);
-                                // one lane of one warp owns each of these sums: the additions keep their order
-                                if ((lane & 15) < left)
-                                    atomicAdd(P.db + ((size_t)blockIdx.x * 4 + q) * 2 * P.F + (lane < 16 ? 0 : P.F) + col + (lane & 15), s);
+                                for (int i = 0; i < CH; ++i)
+                                    *reinterpret_cast<uint4*>(buf + (lane / CH + i * (32 / CH)) * LD * 2 + (lane % CH) * 16) = nx[i];
+                            } else {
+                                rows_in_any<T, SC, LD>(buf, (const T*)P.dh, P.F, row0, P.M, col, P.N, lane);
                             }
                         }
-                    } else {
-                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                        if (row < P.M) {
-                            float v[16];
+                        __syncwarp();
+                    }
+                    if (cc + SC < CW) ask(tile, cc + SC);
+                    else ask(tile + W.step, 0);
+                    if (!some) continue;
+                    uint8_t* mine = buf + lane * LD * 2;
+#pragma unroll 1
+                    for (int s = 0; s < SC; s += 16) {
+                        uint32_t r[16];
+                        tmem_ld16(t0 + cc + s, r);
+                        if (PAIR) {
+                            uint32_t ru[16];
+                            tmem_ld16(t0 + TN + cc + s, ru);
+                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
-                            store16((T*)P.out + (size_t)row * P.ldo + col, v, left, P.vec);
+                            for (int e = 0; e < 16; e += 8) {
+                                float bg[8], bu[8];
+                                *reinterpret_cast<float4*>(bg) = *reinterpret_cast<const float4*>(&sb[0][s + e]);
+                                *reinterpret_cast<float4*>(bg + 4) = *reinterpret_cast<const float4*>(&sb[0][s + e + 4]);
+                                *reinterpret_cast<float4*>(bu) = *reinterpret_cast<const float4*>(&sb[1][s + e]);
+                                *reinterpret_cast<float4*>(bu + 4) = *reinterpret_cast<const float4*>(&sb[1][s + e + 4]);
+                                uint4* at = reinterpret_cast<uint4*>(mine + (s + e) * 2);
+                                if (MODE == FWD) {
+                                    float h[8];
+                                    if (P.act == 0) fwd8<0>(r + e, ru + e, bg, bu, h);
+                                    else if (P.act == 1) fwd8<1>(r + e, ru + e, bg, bu, h);
+                                    else if (P.act == 2) fwd8<2>(r + e, ru + e, bg, bu, h);
+                                    else fwd8<3>(r + e, ru + e, bg, bu, h);
+                                    *at = pack8<T>(h);
+                                } else {
+                                    float z[16];
+                                    if (P.act == 0) dz8<T, 0>(r + e, ru + e, bg, bu, *at, z);
+                                    else if (P.act == 1) dz8<T, 1>(r + e, ru + e, bg, bu, *at, z);
+                                    else if (P.act == 2) dz8<T, 2>(r + e, ru + e, bg, bu, *at, z);
+                                    else dz8<T, 3>(r + e, ru + e, bg, bu, *at, z);
+                                    *at = pack8<T>(z);  // dg takes dh's place
+                                    *reinterpret_cast<uint4*>(buf2 + lane * LD * 2 + (s + e) * 2) = pack8<T>(z + 8);
+                                    if (P.db) {
+                                        if (row >= P.M) {  // rows behind the last one add nothing, whatever they hold
+#pragma unroll
+                                            for (int j = 0; j < 16; ++j) z[j] = 0.f;
+                                        }
+                                        const float sum = column_sums(z, lane);
+                                        // one lane of one warp owns each of these sums: the additions keep their order
+                                        const int c = col + s + e + (lane & 7);
+                                        if (lane < 16 && c < P.N)
+                                            atomicAdd(P.db + ((size_t)blockIdx.x * 4 + q) * 2 * P.F + (lane < 8 ? 0 : P.F) + c, sum);
+                                    }
+                                }
+                            }
+                        } else {
+                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                            const float* v = reinterpret_cast<const float*>(r);
+                            *reinterpret_cast<uint4*>(mine + s * 2) = pack8<T>(v);
+                            *reinterpret_cast<uint4*>(mine + s * 2 + 16) = pack8<T>(v + 8);
                         }
                     }
+                    __syncwarp();
+                    // z's rows are padded to whole 16-byte groups
+                    rows_out<T, SC, LD>(buf, (T*)P.out, P.ldo, row0, P.M, col, P.N, MODE == DZ || P.vec, lane);
+                    if (MODE == DZ) rows_out<T, SC, LD>(buf2, (T*)P.out + P.ldo / 2, P.ldo, row0, P.M, col, P.N, true, lane);
+                    __syncwarp();
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;");
                 __syncwarp();
-                if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s32(&S.tempty[acc])) : "memory");
+                if (lane == 0) {
+                    if (CG == 1)
+                        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s32(&S.tempty[acc])) : "memory");
+                    else
+                        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(acc ? tempty1 : tempty0)
+                                     : "memory");
+                }
                 if (++acc == 2) { acc = 0; accph ^= 1u; }
             }
         }
@@ -477,31 +637,42 @@ __global__ void __launch_bounds__(NTH, 1) k_ff(const __grid_constant__ Args P) {
     if (!ok) {
         S.stop = 1;
         atomicExch(&g_err, 1);
+        if (warp == 0)  // give loads in flight 0.1 s to land
+            for (int i = 0; i < 100; ++i) __nanosleep(1000000);
     }
     asm volatile("tcgen05.fence::before_thread_sync;");
     __syncthreads();
+    if (CG > 1) cluster_sync();  // neither CTA leaves while the other reads its memory or arrives on its barriers
     asm volatile("tcgen05.fence::after_thread_sync;");
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN));
+    if (warp == 0) {
+        __syncwarp();
+        if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN));
+        else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN));
+    }
 }
 
 // dW from the partial tiles: tile t is the sum of the slots b + t of the CTAs whose shares of a block's units meet it,
 // in the order of b.  One thread, 4 columns; grid: (rows of a tile) x tiles.
-template <class T, int BN>
+template <class T, int BN, int CG>
 __global__ void __launch_bounds__(256) k_dw_sum(const float* part, T* dw, int F, int K, int tile0, int ntp, int blk, int ctas,
                                                 int ntn) {
-    constexpr int C4 = BN / 4;
+    constexpr int C4 = BN / 4, R = BM * CG;
     const int t = blockIdx.y, idx = blockIdx.x * 256 + threadIdx.x, r = idx / C4, c = (idx % C4) * 4;
     const int tile = tile0 + t, half_tiles = (F + BM - 1) / BM;
-    const int mt = tile / ntn, up = mt >= half_tiles, f = (up ? mt - half_tiles : mt) * BM + r, k = (tile % ntn) * BN + c;
+    const int mt = (tile / ntn) * CG + r / BM, up = mt >= half_tiles;
+    const int f = (up ? mt - half_tiles : mt) * BM + r % BM, k = (tile % ntn) * BN + c;
+    const int U = ntp * blk, lo = t * blk, hi = lo + blk;  // U x ctas stays below 2^31: 148 tiles, 64 chunks, 148 CTAs
+    int b0 = lo * ctas / U, b1 = hi * ctas / U;
+    while (b0 > 0 && U * b0 / ctas > lo) --b0;             // the CTA whose share holds lo ..
+    while (U * (b0 + 1) / ctas <= lo) ++b0;
+    while (b1 >= ctas || U * b1 / ctas >= hi) --b1;        // .. to the one whose share holds hi - 1
+    after_previous();
     if (f >= F || k >= K) return;
-    const long long U = (long long)ntp * blk, lo = (long long)t * blk, hi = lo + blk;
-    int b = (int)(lo * ctas / U);  // near the first CTA whose share ends behind lo
-    while (b > 0 && U * b / ctas > lo) --b;
-    while (U * (b + 1) / ctas <= lo) ++b;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (; b < ctas && U * b / ctas < hi; ++b) {
-        if (U * (b + 1) / ctas == U * b / ctas) continue;  // an empty share
-        const float4 v = __ldcs(reinterpret_cast<const float4*>(part + ((size_t)(b + t) * BM + r) * BN + c));
+    const float* src = part + ((size_t)t * R + r) * BN + c;
+#pragma unroll 8
+    for (int b = b0; b <= b1; ++b) {
+        const float4 v = __ldcs(reinterpret_cast<const float4*>(src + (size_t)b * R * BN));
         s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
     }
     T* dst = dw + (size_t)(up ? F + f : f) * K + k;
@@ -519,7 +690,9 @@ __global__ void __launch_bounds__(1024) k_db_sum(const float* part, float* db, i
     __shared__ double sh[32][33];
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5, col = blockIdx.x * 32 + x;
     double s = 0.0;
+    after_previous();
     if (col < n)
+#pragma unroll 4
         for (int r = y; r < rows; r += 32) s += part[(size_t)r * n + col];
     sh[y][x] = s;
     __syncthreads();
@@ -529,19 +702,97 @@ __global__ void __launch_bounds__(1024) k_db_sum(const float* part, float* db, i
     if (x == 0 && blockIdx.x * 32 + y < n) db[blockIdx.x * 32 + y] = (float)v;
 }
 
-// rows of 16-bit numbers copied to rows of `ldd` (a multiple of 8), zeros behind the n-th
-__global__ void __launch_bounds__(256) k_pad(const uint16_t* src, long long ld, uint16_t* dst, int ldd, int n, long long rows) {
+// rows of 16-bit numbers copied to rows of `ldd` (a multiple of 8), zeros behind the n-th; two matrices in one launch
+struct PadJob {
+    const uint16_t* src;
+    uint16_t* dst;
+    long long ld, rows;
+};
+__global__ void __launch_bounds__(256) k_pad(PadJob a, PadJob b, int ldd, int n) {
+    after_previous();
     const int groups = ldd / 8;
-    const long long total = rows * groups;
+    const long long na = a.rows * groups, total = na + b.rows * groups;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const long long r = i / groups;
-        const int c = (int)(i % groups) * 8;
+        const PadJob& j = i < na ? a : b;
+        const long long e = i < na ? i : i - na, r = e / groups;
+        const int c = (int)(e % groups) * 8;
         uint16_t v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = c + j < n ? src[r * ld + c + j] : (uint16_t)0;
+        for (int q = 0; q < 8; ++q) v[q] = c + q < n ? j.src[r * j.ld + c + q] : (uint16_t)0;
         uint4 o;
         memcpy(&o, v, 16);
-        *reinterpret_cast<uint4*>(dst + r * ldd + c) = o;
+        *reinterpret_cast<uint4*>(j.dst + r * ldd + c) = o;
+    }
+}
+
+// The forward pass of a few rows (a world or some asking for their next action): the weights' bytes are the work, and
+// 128-row tiles would leave it to F / 32 CTAs at most.  One warp an output: it reads row f of Wg and of Wu once, 16 bytes
+// a lane (VEC; single numbers where rows start anywhere), the rows of X come from L1.  R rows at a time.
+template <class T, int R, bool VEC>
+__global__ void __launch_bounds__(256) k_ff_rows(int M, int K, int F, int act, const T* __restrict__ X, long long ldx,
+                                                 const T* __restrict__ W, long long ldw, const float* __restrict__ bias,
+                                                 T* __restrict__ h) {
+    const int f = (blockIdx.x * 256 + threadIdx.x) >> 5, lane = threadIdx.x & 31;
+    after_previous();
+    if (f >= F) return;
+    const T *wg = W + (size_t)f * ldw, *wu = W + (size_t)(F + f) * ldw;
+    for (int m0 = 0; m0 < M; m0 += R) {
+        float g[R], u[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) g[r] = u[r] = 0.f;
+        if constexpr (VEC) {
+#pragma unroll 4
+            for (int k = lane * 8; k < K; k += 256) {
+                const uint4 a = __ldg(reinterpret_cast<const uint4*>(wg + k)), c = __ldg(reinterpret_cast<const uint4*>(wu + k));
+                const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, cw[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    if (m0 + r >= M) break;
+                    const uint4 x = __ldg(reinterpret_cast<const uint4*>(X + (m0 + r) * ldx + k));
+                    const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 p = Half2<T>::unpack(aw[j]), q = Half2<T>::unpack(cw[j]), y = Half2<T>::unpack(xw[j]);
+                        g[r] = fmaf(p.x, y.x, g[r]);
+                        g[r] = fmaf(p.y, y.y, g[r]);
+                        u[r] = fmaf(q.x, y.x, u[r]);
+                        u[r] = fmaf(q.y, y.y, u[r]);
+                    }
+                }
+            }
+        } else {
+#pragma unroll 4
+            for (int k = lane; k < K; k += 32) {
+                const float p = Half2<T>::f(wg[k]), q = Half2<T>::f(wu[k]);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    if (m0 + r >= M) break;
+                    const float y = Half2<T>::f(X[(m0 + r) * ldx + k]);
+                    g[r] = fmaf(p, y, g[r]);
+                    u[r] = fmaf(q, y, u[r]);
+                }
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                g[r] += __shfl_xor_sync(0xffffffffu, g[r], o);
+                u[r] += __shfl_xor_sync(0xffffffffu, u[r], o);
+            }
+        }
+        const float bg = bias ? bias[f] : 0.f, bu = bias ? bias[F + f] : 0.f;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            if (lane != r || m0 + r >= M) continue;
+            float a, d;
+            const float x = g[r] + bg;
+            if (act == 0) act1<0, false>(x, a, d);
+            else if (act == 1) act1<1, false>(x, a, d);
+            else if (act == 2) act1<2, false>(x, a, d);
+            else act1<3, false>(x, a, d);
+            h[(size_t)(m0 + r) * F + f] = Half2<T>::one(a * (u[r] + bu));
+        }
     }
 }
 
@@ -558,63 +809,90 @@ static bool map2d(CUtensorMap* m, int type, const void* base, long long cols, lo
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// launches that may start while their predecessor in the stream ends (after_previous); cg CTAs a cluster
+template <class... P, class... A>
+static cudaError_t go(int cg, void (*k)(P...), dim3 grid, int block, int smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid; cfg.blockDim = block; cfg.dynamicSmemBytes = smem; cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cg; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = cg > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, k, args...);
+}
+
 // the shared-memory limit is a property of (function, device)
-template <class T, int MODE, int BN>
-static cudaError_t launch(const Args& P, int grid, cudaStream_t st) {
+template <class T, int MODE, int BN, int CG>
+static cudaError_t launch(const Args& P, int groups, cudaStream_t st) {
     static std::once_flag once[64];
     static cudaError_t rc[64];
+    constexpr int smem = smem_bytes<MODE, BN, CG>();
+    static_assert(smem <= 227 * 1024, "shared memory of a CTA");
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     std::call_once(once[dev], [dev]() {
-        rc[dev] = cudaFuncSetAttribute(k_ff<T, MODE, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<BN>());
+        rc[dev] = cudaFuncSetAttribute(k_ff<T, MODE, BN, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     });
     if (rc[dev] != cudaSuccess) return rc[dev];
-    k_ff<T, MODE, BN><<<grid, NTH, smem_bytes<BN>(), st>>>(P);
-    return cudaGetLastError();
+    return go(CG, k_ff<T, MODE, BN, CG>, dim3(groups * CG), Cfg<MODE, BN, CG>::NTH, smem, st, P);
 }
 
-static bool needs_pad(const void* p, long long ld, int cols) { return cols % 8 || ld % 8 || ((uintptr_t)p & 15); }
+// TMA wants rows on 16-byte boundaries
+static bool needs_pad(const void* p, long long ld) { return ld % 8 || ((uintptr_t)p & 15); }
 static long long up16(long long b) { return (b + 255) & ~255ll; }
 static int pad8(int n) { return (n + 7) & ~7; }
+
+constexpr int ROWS_MAX = 4;  // rows up to which the forward pass goes by k_ff_rows
+
+// Columns of B a tile, for `cols` output columns that B has `per` of for each: 256 on pairs of CTAs (cg 2) where that
+// gives every pair a tile, else 128 or 64 on single ones, the narrower the fewer tiles there are.
+struct Shape {
+    int bn, cg;
+};
+static Shape tile_shape(int M, int cols, int per, int nsm) {
+    auto tiles = [&](int rows, int bn) { return (long long)((M + rows - 1) / rows) * ((cols * per + bn - 1) / bn); };
+    if (cols * per > 128 && tiles(2 * BM, 256) * 2 >= nsm) return {256, 2};
+    if (cols * per > 64 && tiles(BM, 128) * 2 > nsm) return {128, 1};
+    return {64, 1};
+}
 
 struct Plan {
     long long xp, wp, z, db, part, total;  // offsets in the workspace
     bool padx, padw;
-    int dw_bn, tiles, passes, ntp, ctas, blk;
+    Shape dw;
+    int tiles, passes, ntp, groups, blk;
 };
-// DW: passes of at most one tile a CTA (then a CTA's share meets two tiles at most)
-static Plan plan(int M, int K, int F, const void* X, long long ldx, const void* W, int backward, int nsm) {
+// DW: passes of at most one tile a group of CTAs (then its share meets two tiles at most)
+static Plan plan(int M, int K, int F, const void* X, long long ldx, const void* W, long long ldw, int backward, int nsm) {
     Plan L = {};
     long long o = 0;
-    L.padx = needs_pad(X, ldx, K);
-    L.padw = needs_pad(W, K, K);
+    if (!backward && M <= ROWS_MAX) return L;
+    L.padx = needs_pad(X, ldx);
+    L.padw = needs_pad(W, ldw);
     auto take = [&](long long bytes) { const long long at = o; o += up16(bytes); return at; };
     L.xp = take(L.padx ? (long long)M * pad8(K) * 2 : 0);
     L.wp = take(L.padw ? 2ll * F * pad8(K) * 2 : 0);
     if (backward) {
         L.z = take((long long)M * 2 * pad8(F) * 2);
         L.db = take((long long)nsm * 4 * 2 * F * 4);
-        L.dw_bn = K <= 128 ? 128 : 256;
-        L.tiles = 2 * ((F + BM - 1) / BM) * ((K + L.dw_bn - 1) / L.dw_bn);
-        L.passes = (L.tiles + nsm - 1) / nsm;
+        L.dw = K <= 64 ? Shape{64, 1} : K <= 128 ? Shape{128, 1} : Shape{256, 2};
+        const int all = nsm / L.dw.cg;
+        L.tiles = 2 * ((F + BM - 1) / BM) / L.dw.cg * ((K + L.dw.bn - 1) / L.dw.bn);
+        L.passes = (L.tiles + all - 1) / all;
         L.ntp = (L.tiles + L.passes - 1) / L.passes;
         const int nk = (M + BK - 1) / BK;
         L.blk = nk < DW_BLOCK ? nk : DW_BLOCK;
         const long long units = (long long)L.ntp * L.blk;
-        L.ctas = (int)(units < nsm ? units : nsm);
-        L.part = take((long long)(L.ctas + L.ntp) * BM * L.dw_bn * 4);
+        // four chunks a share at least: below that its partial tile costs more than its products
+        L.groups = (int)std::min<long long>(all, std::max<long long>(L.ntp, units / 4));
+        L.part = take((long long)(L.groups + L.ntp) * L.dw.cg * BM * L.dw.bn * 4);
     }
     L.total = o;
     return L;
-}
-
-static cudaError_t pad(const void* src, long long ld, void* dst, int cols, long long rows, cudaStream_t st) {
-    const long long n = rows * (pad8(cols) / 8);
-    const int grid = (int)std::min<long long>((n + 255) / 256, 148 * 16);
-    k_pad<<<grid, 256, 0, st>>>((const uint16_t*)src, ld, (uint16_t*)dst, pad8(cols), cols, rows);
-    return cudaGetLastError();
 }
 
 struct Call {
@@ -622,6 +900,7 @@ struct Call {
     const void* X;
     long long ldx;
     const void* W;
+    long long ldw;
     const float* b;
     uint8_t* ws;
     cudaStream_t st;
@@ -629,50 +908,78 @@ struct Call {
 };
 
 static cudaError_t operands(Call& c, const Plan& L) {
-    cudaError_t e = cudaSuccess;
+    if (!L.padx && !L.padw) return cudaSuccess;
+    const int ldd = pad8(c.K);
+    PadJob a = {}, b = {};
     if (L.padx) {
-        e = pad(c.X, c.ldx, c.ws + L.xp, c.K, c.M, c.st);
-        c.X = c.ws + L.xp;
-        c.ldx = pad8(c.K);
+        a = {(const uint16_t*)c.X, (uint16_t*)(c.ws + L.xp), c.ldx, c.M};
+        c.X = a.dst;
+        c.ldx = ldd;
     }
-    if (L.padw && e == cudaSuccess) {
-        e = pad(c.W, c.K, c.ws + L.wp, c.K, 2ll * c.F, c.st);
-        c.W = c.ws + L.wp;
+    if (L.padw) {
+        b = {(const uint16_t*)c.W, (uint16_t*)(c.ws + L.wp), c.ldw, 2ll * c.F};
+        c.W = b.dst;
+        c.ldw = ldd;
     }
-    return e;
+    const long long n = (a.rows + b.rows) * (ldd / 8);
+    return go(1, k_pad, dim3((unsigned)std::min<long long>((n + 255) / 256, c.nsm * 16)), 256, 0, c.st, a, b, ldd, c.K);
+}
+
+template <class T, int MODE>
+static cudaError_t pair_tiles(const Call& c, Args P, int* ctas) {
+    const Shape sh = tile_shape(c.M, c.F, 2, c.nsm);
+    const int tn = sh.bn / 2, rows = BM * sh.cg;
+    if (!map2d(&P.a0, c.type, c.X, c.K, c.M, c.ldx, BM) || !map2d(&P.b0, c.type, c.W, c.K, c.F, c.ldw, tn) ||
+        !map2d(&P.b1, c.type, (const T*)c.W + c.F * c.ldw, c.K, c.F, c.ldw, tn))
+        return cudaErrorInvalidValue;
+    P.M = c.M; P.N = c.F; P.F = c.F; P.act = c.act; P.bias = c.b;
+    P.nk = (c.K + BK - 1) / BK;
+    const int groups = (int)std::min<long long>((long long)((c.M + rows - 1) / rows) * ((c.F + tn - 1) / tn), c.nsm / sh.cg);
+    *ctas = groups * sh.cg;
+    if (MODE == DZ && P.db) {
+        cudaError_t e = cudaMemsetAsync(P.db, 0, (size_t)*ctas * 4 * 2 * c.F * 4, c.st);
+        if (e != cudaSuccess) return e;
+    }
+    if (sh.bn == 64) return launch<T, MODE, 64, 1>(P, groups, c.st);
+    if (sh.bn == 128) return launch<T, MODE, 128, 1>(P, groups, c.st);
+    return launch<T, MODE, 256, 2>(P, groups, c.st);
 }
 
 template <class T>
 static cudaError_t forward(Call c, const Plan& L, void* h) {
+    if (c.M <= ROWS_MAX) {
+        const bool vec = c.K % 8 == 0 && !needs_pad(c.X, c.ldx) && !needs_pad(c.W, c.ldw);
+        auto rows = [&](auto k) {
+            return go(1, k, dim3((c.F + 7) / 8), 256, 0, c.st, c.M, c.K, c.F, c.act, (const T*)c.X, c.ldx, (const T*)c.W, c.ldw, c.b,
+                      (T*)h);
+        };
+        if (c.M == 1) return vec ? rows(k_ff_rows<T, 1, true>) : rows(k_ff_rows<T, 1, false>);
+        return vec ? rows(k_ff_rows<T, 4, true>) : rows(k_ff_rows<T, 4, false>);
+    }
     cudaError_t e = operands(c, L);
     if (e != cudaSuccess) return e;
-    const long long ldw = L.padw ? pad8(c.K) : c.K;
     Args P = {};
-    if (!map2d(&P.a0, c.type, c.X, c.K, c.M, c.ldx, BM) || !map2d(&P.b0, c.type, c.W, c.K, c.F, ldw, 128) ||
-        !map2d(&P.b1, c.type, (const T*)c.W + c.F * ldw, c.K, c.F, ldw, 128))
-        return cudaErrorInvalidValue;
-    P.M = c.M; P.N = c.F; P.F = c.F; P.act = c.act; P.bias = c.b;
-    P.nk = (c.K + BK - 1) / BK;
     P.out = h; P.ldo = c.F;
     P.vec = c.F % 8 == 0 && ((uintptr_t)h & 15) == 0;
-    const long long tiles = (long long)((c.M + BM - 1) / BM) * ((c.F + 127) / 128);
-    return launch<T, FWD, 256>(P, (int)std::min<long long>(tiles, c.nsm), c.st);
+    int ctas;
+    return pair_tiles<T, FWD>(c, P, &ctas);
 }
 
-template <class T, int BN>
+template <class T, int BN, int CG>
 static cudaError_t dw_passes(const Call& c, const Plan& L, Args P, void* dw, int dw_type) {
     const int ntn = (c.K + BN - 1) / BN;
     for (int t0 = 0; t0 < L.tiles; t0 += L.ntp) {
         P.tile0 = t0;
         P.ntp = std::min(L.ntp, L.tiles - t0);
-        // as many CTAs as the full passes: a share never exceeds one tile
-        const int ctas = (int)std::min<long long>((long long)P.ntp * L.blk, L.ctas);
-        cudaError_t e = launch<T, DW, BN>(P, ctas, c.st);
+        const int groups = (int)std::min<long long>((long long)P.ntp * L.blk, L.groups);
+        static_assert(148ll * DW_BLOCK * 148 < (1ll << 31), "k_dw_sum's products");
+        cudaError_t e = launch<T, DW, BN, CG>(P, groups, c.st);
         if (e != cudaSuccess) return e;
-        const dim3 grid(BM * BN / 4 / 256, P.ntp);
-        if (dw_type == 0) k_dw_sum<float, BN><<<grid, 256, 0, c.st>>>((const float*)P.out, (float*)dw, c.F, c.K, t0, P.ntp, L.blk, ctas, ntn);
-        else k_dw_sum<T, BN><<<grid, 256, 0, c.st>>>((const float*)P.out, (T*)dw, c.F, c.K, t0, P.ntp, L.blk, ctas, ntn);
-        e = cudaGetLastError();
+        const dim3 grid(CG * BM * BN / 4 / 256, P.ntp);
+        const float* part = (const float*)P.out;
+        e = dw_type == 0
+                ? go(1, k_dw_sum<float, BN, CG>, grid, 256, 0, c.st, part, (float*)dw, c.F, c.K, t0, P.ntp, L.blk, groups, ntn)
+                : go(1, k_dw_sum<T, BN, CG>, grid, 256, 0, c.st, part, (T*)dw, c.F, c.K, t0, P.ntp, L.blk, groups, ntn);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
@@ -682,48 +989,36 @@ template <class T>
 static cudaError_t backward(Call c, const Plan& L, const void* dh, void* dx, void* dw, int dw_type, float* db) {
     cudaError_t e = operands(c, L);
     if (e != cudaSuccess) return e;
-    const long long ldw = L.padw ? pad8(c.K) : c.K;
     const int Fp = pad8(c.F);
     T* z = (T*)(c.ws + L.z);
-    const T* Wu = (const T*)c.W + c.F * ldw;
+    const T* Wu = (const T*)c.W + c.F * c.ldw;
     {   // z = [dg | du] and the column sums
         Args P = {};
-        if (!map2d(&P.a0, c.type, c.X, c.K, c.M, c.ldx, BM) || !map2d(&P.b0, c.type, c.W, c.K, c.F, ldw, 128) ||
-            !map2d(&P.b1, c.type, Wu, c.K, c.F, ldw, 128))
-            return cudaErrorInvalidValue;
-        P.M = c.M; P.N = c.F; P.F = c.F; P.act = c.act; P.bias = c.b;
-        P.nk = (c.K + BK - 1) / BK;
         P.out = z; P.ldo = 2 * Fp;
         P.dh = dh;
         P.vec = c.F % 8 == 0 && ((uintptr_t)dh & 15) == 0;
-        const long long tiles = (long long)((c.M + BM - 1) / BM) * ((c.F + 127) / 128);
-        const int grid = (int)std::min<long long>(tiles, c.nsm);
-        if (db) {
-            P.db = (float*)(c.ws + L.db);
-            e = cudaMemsetAsync(P.db, 0, (size_t)grid * 4 * 2 * c.F * 4, c.st);
-            if (e != cudaSuccess) return e;
-        }
-        e = launch<T, DZ, 256>(P, grid, c.st);
+        P.db = db ? (float*)(c.ws + L.db) : nullptr;
+        int ctas;
+        e = pair_tiles<T, DZ>(c, P, &ctas);
+        if (e == cudaSuccess && db)
+            e = go(1, k_db_sum, dim3((2 * c.F + 31) / 32), 1024, 0, c.st, (const float*)P.db, db, ctas * 4, 2 * c.F);
         if (e != cudaSuccess) return e;
-        if (db) {
-            k_db_sum<<<(2 * c.F + 31) / 32, 1024, 0, c.st>>>(P.db, db, grid * 4, 2 * c.F);
-            e = cudaGetLastError();
-            if (e != cudaSuccess) return e;
-        }
     }
     if (dx) {
         Args P = {};
         if (!map2d(&P.a0, c.type, z, c.F, c.M, 2 * Fp, BM) || !map2d(&P.a1, c.type, z + Fp, c.F, c.M, 2 * Fp, BM) ||
-            !map2d(&P.b0, c.type, c.W, c.K, c.F, ldw, BK) || !map2d(&P.b1, c.type, Wu, c.K, c.F, ldw, BK))
+            !map2d(&P.b0, c.type, c.W, c.K, c.F, c.ldw, BK) || !map2d(&P.b1, c.type, Wu, c.K, c.F, c.ldw, BK))
             return cudaErrorInvalidValue;
         P.M = c.M; P.N = c.K; P.F = c.F;
         P.nk = 2 * ((c.F + BK - 1) / BK);
         P.out = dx; P.ldo = c.K;
         P.vec = c.K % 8 == 0 && ((uintptr_t)dx & 15) == 0;
-        const int bn = c.K <= 128 ? 128 : 256;
-        const long long tiles = (long long)((c.M + BM - 1) / BM) * ((c.K + bn - 1) / bn);
-        const int grid = (int)std::min<long long>(tiles, c.nsm);
-        e = bn == 128 ? launch<T, DX, 128>(P, grid, c.st) : launch<T, DX, 256>(P, grid, c.st);
+        const Shape sh = tile_shape(c.M, c.K, 1, c.nsm);
+        const int rows = BM * sh.cg;
+        const int groups = (int)std::min<long long>((long long)((c.M + rows - 1) / rows) * ((c.K + sh.bn - 1) / sh.bn), c.nsm / sh.cg);
+        e = sh.bn == 64    ? launch<T, DX, 64, 1>(P, groups, c.st)
+            : sh.bn == 128 ? launch<T, DX, 128, 1>(P, groups, c.st)
+                           : launch<T, DX, 256, 2>(P, groups, c.st);
         if (e != cudaSuccess) return e;
     }
     if (dw) {
@@ -734,7 +1029,9 @@ static cudaError_t backward(Call c, const Plan& L, const void* dh, void* dx, voi
         P.M = c.M; P.N = c.K; P.F = c.F;
         P.nk = (c.M + BK - 1) / BK;
         P.out = c.ws + L.part;
-        e = L.dw_bn == 128 ? dw_passes<T, 128>(c, L, P, dw, dw_type) : dw_passes<T, 256>(c, L, P, dw, dw_type);
+        e = L.dw.bn == 64    ? dw_passes<T, 64, 1>(c, L, P, dw, dw_type)
+            : L.dw.bn == 128 ? dw_passes<T, 128, 1>(c, L, P, dw, dw_type)
+                             : dw_passes<T, 256, 2>(c, L, P, dw, dw_type);
     }
     return e;
 }
@@ -747,12 +1044,12 @@ static bool shape_ok(int M, int K, int F) {
 
 // shared argument checks; 0 when the call can run
 static int check(const char* who, int M, int K, int F, int type, int act, const void* X, long long ldx, const void* W,
-                 const float* b, const void* ws, long long ws_size, int backward, Plan* L, int* nsm) {
+                 long long ldw, const float* b, const void* ws, long long ws_size, int backward, Plan* L, int* nsm) {
     auto bad = [&](const char* what) { set_error(-22, who, what); return -22; };
     if (!shape_ok(M, K, F)) return bad("invalid shape");
     if (type != 1 && type != 2) return bad("type must be 1 (bf16) or 2 (fp16)");
     if (act < 0 || act > 3) return bad("activation must be 0 tanh, 1 ELU, 2 SiLU or 3 GELU");
-    if (ldx < K && M > 1) return bad("row stride below K");
+    if ((ldx < K && M > 1) || ldw < K || ldx > (1ll << 36) || ldw > (1ll << 36)) return bad("row stride below K or too long");
     if (M > 0 && (!X || ((uintptr_t)X & 1))) return bad("null or misaligned X");
     if (!W || ((uintptr_t)W & 1) || ((uintptr_t)b & 3)) return bad("null or misaligned W or b");
     int dev = 0;
@@ -763,7 +1060,7 @@ static int check(const char* who, int M, int K, int F, int type, int act, const 
     if (e == cudaSuccess) e = cudaSetDevice(dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(nsm, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) { set_error((int)e, who, cudaGetErrorString(e)); return -1; }
-    *L = plan(M, K, F, X, ldx, W, backward, *nsm);
+    *L = plan(M, K, F, X, ldx, W, ldw, backward, *nsm);
     if (L->total > 0 && (!ws || ((uintptr_t)ws & 255) || ws_size < L->total))
         return bad("workspace too small or not 256-byte aligned");
     return 0;
@@ -773,18 +1070,19 @@ static int check(const char* who, int M, int K, int F, int type, int act, const 
 
 extern "C" {
 
-long long g1_gated_ff_workspace(int M, int K, int F, const void* X, long long ldx, const void* W, int backward) {
+long long g1_gated_ff_workspace(int M, int K, int F, const void* X, long long ldx, const void* W, long long ldw,
+                                int backward) {
     if (!g1ff::shape_ok(M, K, F)) return 0;
     int dev = 0, nsm = 148;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&nsm, cudaDevAttrMultiProcessorCount, dev);
-    return g1ff::plan(M, K, F, X, ldx, W, backward, nsm).total;
+    return g1ff::plan(M, K, F, X, M == 1 ? g1ff::pad8(K) : ldx, W, ldw, backward, nsm).total;
 }
 
-int g1_gated_ff(int M, int K, int F, int type, int act, const void* X, long long ldx, const void* W, const float* b, void* h,
-                void* ws, long long ws_size, void* stream) {
+int g1_gated_ff(int M, int K, int F, int type, int act, const void* X, long long ldx, const void* W, long long ldw,
+                const float* b, void* h, void* ws, long long ws_size, void* stream) {
     g1ff::Plan L;
-    g1ff::Call c = {M, K, F, type, act, X, M == 1 ? (long long)K : ldx, W, b, (uint8_t*)ws, (cudaStream_t)stream, 148};
-    const int rc = g1ff::check("g1_gated_ff", M, K, F, type, act, X, c.ldx, W, b, ws, ws_size, 0, &L, &c.nsm);
+    g1ff::Call c = {M, K, F, type, act, X, M == 1 ? g1ff::pad8(K) : ldx, W, ldw, b, (uint8_t*)ws, (cudaStream_t)stream, 148};
+    const int rc = g1ff::check("g1_gated_ff", M, K, F, type, act, X, c.ldx, W, ldw, b, ws, ws_size, 0, &L, &c.nsm);
     if (rc) return rc;
     if (M > 0 && (!h || ((uintptr_t)h & 1))) { set_error(-22, "g1_gated_ff", "null or misaligned h"); return -22; }
     if (M == 0) return 0;
@@ -794,11 +1092,11 @@ int g1_gated_ff(int M, int K, int F, int type, int act, const void* X, long long
 }
 
 int g1_gated_ff_backward(int M, int K, int F, int type, int act, const void* dh, const void* X, long long ldx, const void* W,
-                         const float* b, void* dx, void* dw, int dw_type, float* db, void* ws, long long ws_size,
+                         long long ldw, const float* b, void* dx, void* dw, int dw_type, float* db, void* ws, long long ws_size,
                          void* stream) {
     g1ff::Plan L;
-    g1ff::Call c = {M, K, F, type, act, X, M == 1 ? (long long)K : ldx, W, b, (uint8_t*)ws, (cudaStream_t)stream, 148};
-    const int rc = g1ff::check("g1_gated_ff_backward", M, K, F, type, act, X, c.ldx, W, b, ws, ws_size, 1, &L, &c.nsm);
+    g1ff::Call c = {M, K, F, type, act, X, M == 1 ? g1ff::pad8(K) : ldx, W, ldw, b, (uint8_t*)ws, (cudaStream_t)stream, 148};
+    const int rc = g1ff::check("g1_gated_ff_backward", M, K, F, type, act, X, c.ldx, W, ldw, b, ws, ws_size, 1, &L, &c.nsm);
     if (rc) return rc;
     if ((dw_type != 0 && dw_type != type) || ((uintptr_t)dx & 1) || ((uintptr_t)dw & (dw_type == 0 ? 3 : 1)) ||
         ((uintptr_t)db & 3) || (M > 0 && (!dh || ((uintptr_t)dh & 1)))) {

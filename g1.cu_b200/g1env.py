@@ -7,6 +7,7 @@ The CUDA library is required: importing works on a CPU-only machine, but creatin
 or calling a kernel entry point raises if libg1env.so is missing or no GPU is visible --
 there is no CPU fallback.
 """
+import contextlib
 import ctypes
 import os
 
@@ -60,9 +61,10 @@ SIGNATURES = {
     "g1_obs_prep": (ctypes.c_int, [ctypes.c_longlong, ctypes.c_int] + [_vp] * 6),
     "g1_adv_normalize": (ctypes.c_int, [ctypes.c_longlong, _vp, _vp, _vp]),
     "g1_runnorm_update": (ctypes.c_int, [ctypes.c_int, _vp, _vp, ctypes.c_double, _vp, _vp]),
-    "g1_gated_ff_workspace": (ctypes.c_longlong, [ctypes.c_int] * 3 + [_vp, ctypes.c_longlong, _vp, ctypes.c_int]),
-    "g1_gated_ff": (ctypes.c_int, [ctypes.c_int] * 5 + [_vp, ctypes.c_longlong] + [_vp] * 4 + [ctypes.c_longlong, _vp]),
-    "g1_gated_ff_backward": (ctypes.c_int, [ctypes.c_int] * 5 + [_vp, _vp, ctypes.c_longlong] + [_vp] * 4
+    "g1_gated_ff_workspace": (ctypes.c_longlong, [ctypes.c_int] * 3 + [_vp, ctypes.c_longlong, _vp, ctypes.c_longlong,
+                                                                     ctypes.c_int]),
+    "g1_gated_ff": (ctypes.c_int, [ctypes.c_int] * 5 + [_vp, ctypes.c_longlong] * 2 + [_vp] * 3 + [ctypes.c_longlong, _vp]),
+    "g1_gated_ff_backward": (ctypes.c_int, [ctypes.c_int] * 5 + [_vp] + [_vp, ctypes.c_longlong] * 2 + [_vp] * 3
                              + [ctypes.c_int, _vp, _vp, ctypes.c_longlong, _vp]),
     "g1_gated_ff_status": (ctypes.c_int, []),
     "g1_opt_workspace": (ctypes.c_longlong, [ctypes.c_int]),
@@ -291,55 +293,84 @@ _ACT = {"tanh": 0, "elu": 1, "silu": 2, "gelu": 3}
 _FF_TYPE = {torch.bfloat16: 1, torch.float16: 2}
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(dev):
     """Makes `dev` the current device for the calls within."""
-    return torch.cuda.device(dev)
+    return _HERE if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _stream_of(dev):
+    """torch's current stream on `dev`, as the number that the C-ABI takes"""
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+def _rows(t):
+    """The last axis as the columns of a matrix whose rows do not overlap; a copy only where there is no such view."""
+    m = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    if m.is_contiguous():
+        return m
+    if (m.stride(1) != 1 and m.shape[1] > 1) or (m.shape[0] > 1 and m.stride(0) < m.shape[1]):
+        return m.contiguous()
+    return m
 
 
 def _ff_args(x, w, b, act):
-    """Checked operands of a gated layer: rows [M, K] of x, w [2F, K] in x's type, b [2F] fp32 or None, act code."""
-    if not (x.is_cuda and w.is_cuda and (b is None or b.is_cuda)):
+    """Checked operands of a gated layer: rows [M, K] of x, w [2F, K] in x's type, b [2F] fp32 or None, and the codes of type
+    and activation."""
+    t, code = _FF_TYPE.get(x.dtype), _ACT.get(act)
+    dev = x.device
+    if dev.type != "cuda":
         raise G1Error("a gated layer takes CUDA tensors (no CPU fallback)")
-    if x.dtype not in _FF_TYPE:
+    if t is None:
         raise G1Error(f"a gated layer takes bf16 or fp16 rows, not {str(x.dtype)[6:]}")
     if w.dtype != x.dtype:
         raise G1Error("the weights must be of the rows' type")
-    if act not in _ACT:
+    if code is None:
         raise G1Error(f"unknown activation {act!r} (one of {', '.join(_ACT)})")
     if w.dim() != 2 or w.shape[0] % 2 or not w.numel() or x.dim() < 1 or x.shape[-1] != w.shape[1]:
         raise G1Error("a gated layer takes x [..., K] and w [2F, K]")
-    if b is not None and (b.shape != w.shape[:1] or not b.is_floating_point()):
-        raise G1Error("the bias must be [2F]")
-    if w.device != x.device or (b is not None and b.device != x.device):
+    if w.device != dev or (b is not None and b.device != dev):
         raise G1Error("a gated layer's tensors must be on one device")
-    x2 = x.reshape(-1, x.shape[-1])
-    if x2.stride(1) != 1 and x2.shape[1] > 1 or x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]:
-        x2 = x2.contiguous()
-    if x2.shape[0] > 1 << 30:
-        raise G1Error("too many rows")
-    return x2, w.contiguous(), None if b is None else b.float().contiguous(), _ACT[act]
+    if b is not None:
+        if b.shape != w.shape[:1] or not b.is_floating_point():
+            raise G1Error("the bias must be [2F]")
+        if b.dtype != torch.float32:
+            b = b.float()
+        b = b.contiguous()
+    return _rows(x), _rows(w), b, t, code
 
 
-def _ff_ws(lib, x2, w, F, backward):
-    """(rows, K, ld) and the workspace of a call; None where it needs none."""
-    M, K = x2.shape
-    ld = x2.stride(0) if M > 1 else K
-    n = lib.g1_gated_ff_workspace(M, K, F, _dp(x2), ld, _dp(w), backward)
-    return M, K, ld, n, torch.empty(n, dtype=torch.uint8, device=x2.device) if n else None
+def _ff_ws(lib, x, w, F, backward):
+    """(M, K, address and row stride of x and of w), the bytes of the call's workspace and the workspace"""
+    M, K = x.shape
+    px, ldx, pw, ldw = x.data_ptr(), x.stride(0) if M > 1 else K, w.data_ptr(), w.stride(0)
+    n = 0
+    if backward or (px | pw) & 15 or (ldx | ldw) & 7:   # else nothing has to be copied
+        n = lib.g1_gated_ff_workspace(M, K, F, px, ldx, pw, ldw, backward)
+        if n < 0 or M > 1 << 30:
+            raise G1Error("too many rows")
+    return M, K, px, ldx, pw, ldw, n, torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
 
 
 def gated_ff_device(x, w, b=None, act="silu"):
     """One gated layer, h = act(x Wg^T + bg) * (x Wu^T + bu) (g1_gated_ff): x [..., K] bf16 or fp16, w [2F, K] of the
     same type (the F gate rows, then the F up rows), b [2F] or None, act "tanh", "elu", "silu" or "gelu" (erf).
     Returns h [..., F] in x's type, on torch's current stream.  Rows may be strided; rows or weights that do
-    not start on 16-byte boundaries (K not a multiple of 8) are copied first."""
+    not start on 16-byte boundaries (a row stride that is no multiple of 8) are copied first."""
     lib = load_library()
-    x2, w, b, code = _ff_args(x, w, b, act)
+    x2, w, b, t, code = _ff_args(x, w, b, act)
     F = w.shape[0] // 2
-    with _on(x.device):
-        M, K, ld, n, ws = _ff_ws(lib, x2, w, F, 0)
-        h = torch.empty(x.shape[:-1] + (F,), dtype=x.dtype, device=x.device)
-        if lib.g1_gated_ff(M, K, F, _FF_TYPE[x.dtype], code, _dp(x2), ld, _dp(w), _dp(b), _dp(h), _dp(ws), n, _stream()):
+    dev = x2.device
+    with _on(dev):
+        M, K, px, ldx, pw, ldw, n, ws = _ff_ws(lib, x2, w, F, 0)
+        h = torch.empty(x.shape[:-1] + (F,), dtype=x.dtype, device=dev)
+        if lib.g1_gated_ff(M, K, F, t, code, px, ldx, pw, ldw, _addr(b), h.data_ptr(), _addr(ws), n, _stream_of(dev)):
             _check()
     return h
 
@@ -349,22 +380,23 @@ def gated_ff_backward_device(dh, x, w, b=None, act="silu", need=(True, True, Tru
     or fp32), db [2F] fp32; None where `need` (dx, dw, db) says so.  Nothing of the forward pass but its inputs
     is needed.  dg and du are rounded to x's type before the products with W and x, but not in db."""
     lib = load_library()
-    x2, w, b, code = _ff_args(x, w, b, act)
+    x2, w, b, t, code = _ff_args(x, w, b, act)
     F = w.shape[0] // 2
-    dw_dtype = x.dtype if dw_dtype is None else dw_dtype
-    if dw_dtype not in (x.dtype, torch.float32):
+    dev = x2.device
+    if dw_dtype is None:
+        dw_dtype = x.dtype
+    elif dw_dtype not in (x.dtype, torch.float32):
         raise G1Error("dw is fp32 or of the rows' type")
-    if dh.device != x.device or dh.dtype != x.dtype or tuple(dh.shape) != tuple(x.shape[:-1]) + (F,):
+    if dh.device != dev or dh.dtype != x.dtype or dh.shape != x.shape[:-1] + (F,):
         raise G1Error("dh must be [..., F] on x's device and of its type")
     dh = dh.contiguous()
-    dev = x.device
     with _on(dev):
-        M, K, ld, n, ws = _ff_ws(lib, x2, w, F, 1)
+        M, K, px, ldx, pw, ldw, n, ws = _ff_ws(lib, x2, w, F, 1)
         dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
         dw = torch.empty(2 * F, K, dtype=dw_dtype, device=dev) if need[1] else None
         db = torch.empty(2 * F, dtype=torch.float32, device=dev) if need[2] else None
-        if lib.g1_gated_ff_backward(M, K, F, _FF_TYPE[x.dtype], code, _dp(dh), _dp(x2), ld, _dp(w), _dp(b), _dp(dx),
-                                    _dp(dw), _FF_TYPE.get(dw_dtype, 0), _dp(db), _dp(ws), n, _stream()):
+        if lib.g1_gated_ff_backward(M, K, F, t, code, dh.data_ptr(), px, ldx, pw, ldw, _addr(b), _addr(dx), _addr(dw),
+                                    _FF_TYPE.get(dw_dtype, 0), _addr(db), _addr(ws), n, _stream_of(dev)):
             _check()
     return dx, dw, db
 

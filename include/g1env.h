@@ -176,7 +176,7 @@ int g1_runnorm_update(int dim, float* mean, float* var, double count, const doub
 
 /* extension: one gated policy layer on the tensor cores (tcgen05), beside g1_gemm_bf16_tc's plain one:
  *     h = act(X Wg^T + bg) * (X Wu^T + bu)
- * X [M][K] (row stride ldx), W [2F][K] = [Wg; Wu] row-major, b fp32 [2F] = [bg; bu] or NULL, h [M][F]; X, W, h of one
+ * X [M][K] (row stride ldx), W [2F][K] = [Wg; Wu] (row stride ldw), b fp32 [2F] = [bg; bu] or NULL, h [M][F]; X, W, h of one
  * type: 1 bf16, 2 fp16; fp32 sums, one rounding at the end; act 0 tanh, 1 ELU, 2 SiLU, 3 GELU (erf).  DEVICE
  * pointers on the current device, asynchronous on `stream`, 0 on success.
  *   g1_gated_ff_backward  from dh [M][F]: dx [M][K], dw [2F][K] (dw_type 0 fp32, or the inputs' type), db fp32
@@ -186,11 +186,12 @@ int g1_runnorm_update(int dim, float* mean, float* var, double count, const doub
  * also holds copies of X and W where their rows do not start on 16-byte boundaries).
  *   g1_gated_ff_status    nonzero if a wait of these kernels ran out on the current device since the last call
  *                         (synchronous; clears) */
-long long g1_gated_ff_workspace(int M, int K, int F, const void* X, long long ldx, const void* W, int backward);
-int g1_gated_ff(int M, int K, int F, int type, int act, const void* X, long long ldx, const void* W, const float* b, void* h,
-                void* ws, long long ws_size, void* stream);
+long long g1_gated_ff_workspace(int M, int K, int F, const void* X, long long ldx, const void* W, long long ldw,
+                                int backward);
+int g1_gated_ff(int M, int K, int F, int type, int act, const void* X, long long ldx, const void* W, long long ldw,
+                const float* b, void* h, void* ws, long long ws_size, void* stream);
 int g1_gated_ff_backward(int M, int K, int F, int type, int act, const void* dh, const void* X, long long ldx, const void* W,
-                         const float* b, void* dx, void* dw, int dw_type, float* db, void* ws, long long ws_size,
+                         long long ldw, const float* b, void* dx, void* dw, int dw_type, float* db, void* ws, long long ws_size,
                          void* stream);
 int g1_gated_ff_status(void);
 

@@ -217,11 +217,11 @@ def test_memory_around_the_outputs_stays():
         x, w, b, dh = _make(M, K, F, F16, True, seed=2)
         bufs = {k: torch.full((n + 64,), 7.0, device="cuda", dtype=t) for k, n, t in
                 (("h", M * F, F16), ("dx", M * K, F16), ("dw", 2 * F * K, F16), ("db", 2 * F, torch.float32))}
-        n = lib.g1_gated_ff_workspace(M, K, F, vp(x), K, vp(w), 1)
+        n = lib.g1_gated_ff_workspace(M, K, F, vp(x), K, vp(w), K, 1)
         ws = torch.empty(n, dtype=torch.uint8, device="cuda")
         s = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
-        assert lib.g1_gated_ff(M, K, F, 2, 2, vp(x), K, vp(w), vp(b), vp(bufs["h"]), vp(ws), n, s) == 0
-        assert lib.g1_gated_ff_backward(M, K, F, 2, 2, vp(dh), vp(x), K, vp(w), vp(b), vp(bufs["dx"]), vp(bufs["dw"]), 2,
+        assert lib.g1_gated_ff(M, K, F, 2, 2, vp(x), K, vp(w), K, vp(b), vp(bufs["h"]), vp(ws), n, s) == 0
+        assert lib.g1_gated_ff_backward(M, K, F, 2, 2, vp(dh), vp(x), K, vp(w), K, vp(b), vp(bufs["dx"]), vp(bufs["dw"]), 2,
                                         vp(bufs["db"]), vp(ws), n, s) == 0
         want = [g1env.gated_ff_device(x, w, b), *g1env.gated_ff_backward_device(dh, x, w, b)]
         for k, y in zip(("h", "dx", "dw", "db"), want):
