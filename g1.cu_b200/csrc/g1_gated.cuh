@@ -64,7 +64,7 @@ struct Args {
     const void* dh;              // DZ: [M][F]
     void* out;                   // h [M][F], z [M][2 Fp], dX [M][K], or the fp32 partial tiles
     long long ldo;
-    float* db;                   // DZ: [gridDim][4][2F] column sums, zeroed, or null
+    float* db;                   // DZ: [gridDim][4][2F] column sums, or null
     int tile0, ntp;              // DW: the pass's tiles
     int vec;                     // rows of the output and of dh are 16-byte aligned
 };
@@ -119,32 +119,105 @@ struct Half2<__half> {
     static __device__ __forceinline__ float f(__half a) { return __half2float(a); }
 };
 
-__device__ __forceinline__ float sigmoid(float g) {
-    float r;
-    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-g)));
+// ---- two fp32 numbers an instruction
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 mk(float x, float y) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
     return r;
 }
+__device__ __forceinline__ f2 mk(float2 v) { return mk(v.x, v.y); }
+__device__ __forceinline__ f2 all(float x) { return mk(x, x); }
+__device__ __forceinline__ float2 un(f2 v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ f2 add(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 mul(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 fma(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+// 2^x and 1/x of the special-function unit (2 and 1 units in the last place; results below 2^-126 are 0)
+__device__ __forceinline__ f2 ex2(f2 v) {
+    float2 x = un(v);
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x.x));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x.y));
+    return mk(x);
+}
+__device__ __forceinline__ f2 rcp(f2 v) {
+    float2 x = un(v);
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x.x));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x.y));
+    return mk(x);
+}
+constexpr float LOG2E = 1.4426950408889634f;
 
-// act(g) and, with D, act'(g)
+// act(g) and, with D, act'(g), in about 2^-21 of 1 + |g|; relative to act itself near 0 too.
+//   tanh   1 - 2 / (1 + e^2|g|) with g's sign; its Taylor series to the 7th power where |g| < 0.2 (the rest is 6e-8 of g)
+//   ELU    e^g - 1 below 0; its Taylor series to the 6th power where g > -0.25
+//   SiLU   g s, s = 1 / (1 + e^-g); derivative s + g s (1 - s)
+//   GELU   g Phi(g), derivative Phi(g) + g phi(g); with e = e^(-g^2 / 2) and t = 1 / (1 + p |g| / sqrt 2), Phi(-|g|) is e t P(t) / 2:
+//          Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26 (erf to 1.5e-7), the same e as phi's
+// (CUDA's tanhf, expm1f and erff take 20 to 40 instructions a number, and the epilogue is what bounds DZ.)
 template <int ACT, bool D>
-__device__ __forceinline__ void act1(float g, float& a, float& d) {
+__device__ __forceinline__ void act2(f2 g, f2& a, f2& d) {
+    const f2 one = all(1.f);
     if (ACT == 0) {
-        a = tanhf(g);
-        if (D) d = 1.f - a * a;
+        const float2 x = un(g);
+        const f2 m = mk(fabsf(x.x), fabsf(x.y));
+        const f2 r = rcp(add(ex2(mul(m, all(2.f * LOG2E))), one));
+        const float2 big = un(fma(r, all(-2.f), one));
+        const f2 q = mul(g, g);
+        const float2 ser = un(mul(g, fma(q, fma(q, fma(q, all(-17.f / 315.f), all(2.f / 15.f)), all(-1.f / 3.f)), one)));
+        a = mk(fabsf(x.x) < 0.2f ? ser.x : copysignf(big.x, x.x), fabsf(x.y) < 0.2f ? ser.y : copysignf(big.y, x.y));
+        if (D) {
+            // 1 - tanh^2 keeps its relative size as 4 r (1 - r)
+            d = mul(mul(r, all(4.f)), fma(r, all(-1.f), one));
+        }
     } else if (ACT == 1) {
-        const float e = expm1f(fminf(g, 0.f));
-        a = g > 0.f ? g : e;
-        if (D) d = g > 0.f ? 1.f : e + 1.f;
-        if (g != g) a = d = g;  // fminf drops a NaN
+        const float2 x = un(g);
+        const f2 n = mk(x.x > 0.f ? 0.f : x.x, x.y > 0.f ? 0.f : x.y);  // keeps a NaN
+        const float2 e = un(ex2(mul(n, all(LOG2E))));
+        const float2 s = un(mul(
+            n, fma(n, fma(n, fma(n, fma(n, fma(n, all(1.f / 720.f), all(1.f / 120.f)), all(1.f / 24.f)), all(1.f / 6.f)), all(0.5f)), one)));
+        const float2 nn = un(n);
+        a = mk(x.x > 0.f ? x.x : nn.x > -0.25f ? s.x : e.x - 1.f, x.y > 0.f ? x.y : nn.y > -0.25f ? s.y : e.y - 1.f);
+        if (D) d = mk(e);
     } else if (ACT == 2) {
-        const float s = sigmoid(g);
-        a = g * s;
-        if (D) d = fmaf(a, 1.f - s, s);
+        const f2 s = rcp(add(ex2(mul(g, all(-LOG2E))), one));
+        a = mul(g, s);
+        if (D) d = fma(a, fma(s, all(-1.f), one), s);
     } else {
-        const float c = fmaf(0.5f, erff(g * 0.70710678118654752f), 0.5f);
-        a = g * c;
-        if (D) d = fmaf(g * 0.39894228040143268f, __expf(-0.5f * g * g), c);
+        const float2 x = un(g);
+        const f2 m = mk(fabsf(x.x), fabsf(x.y));
+        const f2 e = ex2(mul(mul(g, g), all(-0.5f * LOG2E)));
+        const f2 t = rcp(fma(m, all(0.3275911f * 0.70710678118654752f), one));
+        const f2 p = fma(t, fma(t, fma(t, fma(t, all(1.061405429f), all(-1.453152027f)), all(1.421413741f)), all(-0.284496736f)),
+                         all(0.254829592f));
+        const float2 c = un(mul(mul(e, all(0.5f)), mul(t, p)));  // Phi(-|g|)
+        const f2 phi = mk(x.x > 0.f ? 1.f - c.x : c.x, x.y > 0.f ? 1.f - c.y : c.y);
+        a = mul(g, phi);
+        if (D) d = fma(mul(g, all(0.39894228040143268f)), e, phi);
     }
+}
+
+// 16 TMEM lanes x 16 columns: lane l holds columns 2 (l % 4), + 1 and 8 further on of rows l / 4 and l / 4 + 8, as
+// r[4 k + 2 i + c] = (row l / 4 + 8 i, column 8 k + 2 (l % 4) + c)
+__device__ __forceinline__ void tmem_ld16x16(uint32_t taddr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
 }
 
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
@@ -202,54 +275,55 @@ __device__ __forceinline__ void rows_out(const uint8_t* buf, T* m, long long ld,
         }
     }
 }
-template <class T, int SC, int LD>
-__device__ __forceinline__ void rows_in_any(uint8_t* buf, const T* m, long long ld, int row0, int M, int col, int N, int lane) {
-    const int c = lane % SC;
-#pragma unroll 8
-    for (int i = 0; i < SC; ++i) {
-        const int r = lane / SC + i * (32 / SC);
-        reinterpret_cast<T*>(buf)[r * LD + c] =
-            row0 + r < M && col + c < N ? m[(size_t)(row0 + r) * ld + col + c] : Half2<T>::one(0.f);
-    }
+// v[0..3] summed over the 8 lanes of equal l % 4: halves of the list change sides twice; lane l gets the sum of
+// v[2 (l / 16) + (l / 8) % 2]
+__device__ __forceinline__ float sums4(const float* v, int lane) {
+    const bool hi = lane & 16, mid = lane & 8;
+    float a = hi ? v[2] : v[0], b = hi ? v[3] : v[1];
+    a += __shfl_xor_sync(0xffffffffu, hi ? v[0] : v[2], 16);
+    b += __shfl_xor_sync(0xffffffffu, hi ? v[1] : v[3], 16);
+    const float s = (mid ? b : a) + __shfl_xor_sync(0xffffffffu, mid ? a : b, 8);
+    return s + __shfl_xor_sync(0xffffffffu, s, 4);
 }
 
-// lane l gets the sum over the warp's lanes of v[l % 16]: halves of the list change sides 4 times
-__device__ __forceinline__ float column_sums(float (&v)[16], int lane) {
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) {
-        const bool up = lane & o;
-#pragma unroll
-        for (int j = 0; j < o; ++j) {
-            const float send = up ? v[j] : v[j + o], keep = up ? v[j + o] : v[j];
-            v[j] = keep + __shfl_xor_sync(0xffffffffu, send, o);
-        }
-    }
-    return v[0] + __shfl_xor_sync(0xffffffffu, v[0], 16);
-}
+__device__ __forceinline__ f2 acc2(const uint32_t* r) { return mk(__uint_as_float(r[0]), __uint_as_float(r[1])); }
 
-// h of 8 columns
+// h of 8 columns of a row
 template <int ACT>
 __device__ __forceinline__ void fwd8(const uint32_t* rg, const uint32_t* ru, const float* bg, const float* bu, float* h) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        float a, d;
-        act1<ACT, false>(__uint_as_float(rg[j]) + bg[j], a, d);
-        h[j] = a * (__uint_as_float(ru[j]) + bu[j]);
+    for (int j = 0; j < 8; j += 2) {
+        f2 a, d;
+        act2<ACT, false>(add(acc2(rg + j), mk(bg[j], bg[j + 1])), a, d);
+        *reinterpret_cast<float2*>(h + j) = un(mul(a, add(acc2(ru + j), mk(bu[j], bu[j + 1]))));
     }
 }
-// z of 8 columns: dg, du.  dh is packed 16-bit pairs
-template <class T, int ACT>
-__device__ __forceinline__ void dz8(const uint32_t* rg, const uint32_t* ru, const float* bg, const float* bu, uint4 dh4,
-                                    float* z) {
-    const uint32_t w[4] = {dh4.x, dh4.y, dh4.z, dh4.w};
+// z of 32 rows x 16 columns: dh in `buf` is replaced by dg, du goes to `buf2`; the column sums over the rows to s[k][]:
+// columns 8 k + 2 (l % 4), + 1 of dg, then of du
+template <class T, int ACT, int LD>
+__device__ __forceinline__ void dz16(const uint32_t (&rg)[2][8], const uint32_t (&ru)[2][8], const float (*sb)[32], int s0,
+                                     uint8_t* buf, uint8_t* buf2, float (&sum)[2][4], int lane) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float2 p = Half2<T>::unpack(w[j / 2]);
-        const float dh = j & 1 ? p.y : p.x;
-        float a, d;
-        act1<ACT, true>(__uint_as_float(rg[j]) + bg[j], a, d);
-        z[j] = dh * (__uint_as_float(ru[j]) + bu[j]) * d;
-        z[8 + j] = dh * a;
+    for (int k = 0; k < 2; ++k) {
+        const int c = s0 + 8 * k + 2 * (lane & 3);
+        const f2 bg = *reinterpret_cast<const f2*>(&sb[0][c]), bu = *reinterpret_cast<const f2*>(&sb[1][c]);
+        f2 sg = 0, su = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int off = (((lane >> 2) + 8 * i) * LD + c) * 2;
+            uint32_t* at = reinterpret_cast<uint32_t*>(buf + off);
+            const f2 dh = mk(Half2<T>::unpack(*at));
+            f2 a, d;
+            act2<ACT, true>(add(acc2(&rg[i / 2][4 * k + 2 * (i & 1)]), bg), a, d);
+            const f2 dg = mul(mul(dh, add(acc2(&ru[i / 2][4 * k + 2 * (i & 1)]), bu)), d), du = mul(dh, a);
+            const float2 x = un(dg), y = un(du);
+            *at = Half2<T>::pack(x.x, x.y);
+            *reinterpret_cast<uint32_t*>(buf2 + off) = Half2<T>::pack(y.x, y.y);
+            sg = add(sg, dg);
+            su = add(su, du);
+        }
+        const float2 x = un(sg), y = un(su);
+        sum[k][0] = x.x; sum[k][1] = x.y; sum[k][2] = y.x; sum[k][3] = y.y;
     }
 }
 template <class T>
@@ -513,10 +587,20 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
             uint8_t* buf2 = S.buf[warp - 2][C::BUFS - 1];
             float(*sb)[32] = S.bias[PAIR ? warp - 2 : 0];
             const uint32_t tempty0 = CG == 1 ? 0 : at_leader(s32(&S.tempty[0])), tempty1 = CG == 1 ? 0 : at_leader(s32(&S.tempty[1]));
+            // column (counted from a 16-column step's first) that this lane's sums are of, in its 8-column half
+            const int mycol = 2 * (lane & 3) + ((lane >> 3) & 1);
+            float* mydb = MODE == DZ && P.db && !(lane & 4) ? P.db + ((size_t)blockIdx.x * 4 + q) * 2 * P.F + (lane & 16 ? P.F : 0)
+                                                            : nullptr;
+            if (MODE == DZ && mydb) {
+                // the sums start at 0; the additions below are the same thread's, so they come after
+                for (int c = part * CW + mycol; c < P.N; c += TN)
+                    for (int e = 0; e < CW; e += 8)
+                        if (c + e < P.N) mydb[c + e] = 0.f;
+            }
             // the bias (a column a lane) and dh (as rows_out lays out its accesses) of a step are asked for one step ahead,
             // a tile's first before the wait for its products
             constexpr int CH = SC / 8;
-            uint4 nx[CH];
+            union { uint4 v[CH]; uint32_t w[4 * CH]; } nx;
             float nbg = 0.f, nbu = 0.f;
             auto ask = [&](int tile, int cc) {
                 if (!PAIR || tile >= ntiles) return;
@@ -526,14 +610,27 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                     nbg = __ldg(P.bias + col + lane);
                     nbu = __ldg(P.bias + P.F + col + lane);
                 }
-                if (MODE == DZ && P.vec) {
-                    const int row0 = ((tile / ntn) * CG + rank) * BM + 32 * q, ch = lane % CH;
+                if (MODE == DZ) {
+                    const int row0 = ((tile / ntn) * CG + rank) * BM + 32 * q;
+                    const T* dh = (const T*)P.dh;
+                    if (P.vec) {
+                        const int ch = lane % CH;
 #pragma unroll
-                    for (int i = 0; i < CH; ++i) {
-                        const int r = row0 + lane / CH + i * (32 / CH);
-                        nx[i] = r < P.M && col + 8 * ch < P.N
-                                    ? __ldcs(reinterpret_cast<const uint4*>((const T*)P.dh + (size_t)r * P.F + col + 8 * ch))
-                                    : make_uint4(0, 0, 0, 0);
+                        for (int i = 0; i < CH; ++i) {
+                            const int r = row0 + lane / CH + i * (32 / CH);
+                            nx.v[i] = r < P.M && col + 8 * ch < P.N
+                                          ? __ldcs(reinterpret_cast<const uint4*>(dh + (size_t)r * P.F + col + 8 * ch))
+                                          : make_uint4(0, 0, 0, 0);
+                        }
+                    } else {  // one number a lane and access, two packed
+                        const uint16_t* d16 = reinterpret_cast<const uint16_t*>(dh);
+                        const int c = col + lane % SC;
+#pragma unroll
+                        for (int i = 0; i < SC; ++i) {
+                            const int r = row0 + lane / SC + i * (32 / SC);
+                            const uint32_t x = r < P.M && c < P.N ? d16[(size_t)r * P.F + c] : 0;
+                            nx.w[i / 2] = i & 1 ? nx.w[i / 2] | (x << 16) : x;
+                        }
                     }
                 }
             };
@@ -541,7 +638,7 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
             for (int tile = W.tile; tile < ntiles; tile += W.step) {
                 if (!wait(&S.tfull[acc], accph)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;");
-                const int row0 = ((tile / ntn) * CG + rank) * BM + 32 * q, row = row0 + lane;
+                const int row0 = ((tile / ntn) * CG + rank) * BM + 32 * q;
                 const uint32_t t0 = tl + acc * BN + part * CW;
 #pragma unroll 1
                 for (int cc = 0; cc < CW; cc += SC) {
@@ -553,9 +650,12 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                             if (P.vec) {
 #pragma unroll
                                 for (int i = 0; i < CH; ++i)
-                                    *reinterpret_cast<uint4*>(buf + (lane / CH + i * (32 / CH)) * LD * 2 + (lane % CH) * 16) = nx[i];
+                                    *reinterpret_cast<uint4*>(buf + (lane / CH + i * (32 / CH)) * LD * 2 + (lane % CH) * 16) = nx.v[i];
                             } else {
-                                rows_in_any<T, SC, LD>(buf, (const T*)P.dh, P.F, row0, P.M, col, P.N, lane);
+#pragma unroll
+                                for (int i = 0; i < SC; ++i)
+                                    reinterpret_cast<uint16_t*>(buf)[(lane / SC + i * (32 / SC)) * LD + lane % SC] =
+                                        (uint16_t)(nx.w[i / 2] >> (16 * (i & 1)));
                             }
                         }
                         __syncwarp();
@@ -566,53 +666,52 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                     uint8_t* mine = buf + lane * LD * 2;
 #pragma unroll 1
                     for (int s = 0; s < SC; s += 16) {
+                        if (MODE == DZ) {
+                            uint32_t rg[2][8], ru[2][8];
+                            tmem_ld16x16(t0 + cc + s, rg[0]);
+                            tmem_ld16x16(t0 + (16u << 16) + cc + s, rg[1]);
+                            tmem_ld16x16(t0 + TN + cc + s, ru[0]);
+                            tmem_ld16x16(t0 + (16u << 16) + TN + cc + s, ru[1]);
+                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                            float sum[2][4];
+                            if (P.act == 0) dz16<T, 0, LD>(rg, ru, sb, s, buf, buf2, sum, lane);
+                            else if (P.act == 1) dz16<T, 1, LD>(rg, ru, sb, s, buf, buf2, sum, lane);
+                            else if (P.act == 2) dz16<T, 2, LD>(rg, ru, sb, s, buf, buf2, sum, lane);
+                            else dz16<T, 3, LD>(rg, ru, sb, s, buf, buf2, sum, lane);
+                            if (P.db) {  // rows behind the last one have dh = 0
+#pragma unroll
+                                for (int k = 0; k < 2; ++k) {
+                                    const float v = sums4(sum[k], lane);
+                                    // one lane of one warp owns each of these sums: the additions keep their order
+                                    const int c = col + s + 8 * k + mycol;
+                                    if (mydb && c < P.N) atomicAdd(mydb + c, v);
+                                }
+                            }
+                            continue;
+                        }
                         uint32_t r[16];
                         tmem_ld16(t0 + cc + s, r);
-                        if (PAIR) {
-                            uint32_t ru[16];
-                            tmem_ld16(t0 + TN + cc + s, ru);
-                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        uint32_t ru[16];
+                        if (MODE == FWD) tmem_ld16(t0 + TN + cc + s, ru);
+                        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-                            for (int e = 0; e < 16; e += 8) {
+                        for (int e = 0; e < 16; e += 8) {
+                            float h[8];
+                            if (MODE == FWD) {
                                 float bg[8], bu[8];
                                 *reinterpret_cast<float4*>(bg) = *reinterpret_cast<const float4*>(&sb[0][s + e]);
                                 *reinterpret_cast<float4*>(bg + 4) = *reinterpret_cast<const float4*>(&sb[0][s + e + 4]);
                                 *reinterpret_cast<float4*>(bu) = *reinterpret_cast<const float4*>(&sb[1][s + e]);
                                 *reinterpret_cast<float4*>(bu + 4) = *reinterpret_cast<const float4*>(&sb[1][s + e + 4]);
-                                uint4* at = reinterpret_cast<uint4*>(mine + (s + e) * 2);
-                                if (MODE == FWD) {
-                                    float h[8];
-                                    if (P.act == 0) fwd8<0>(r + e, ru + e, bg, bu, h);
-                                    else if (P.act == 1) fwd8<1>(r + e, ru + e, bg, bu, h);
-                                    else if (P.act == 2) fwd8<2>(r + e, ru + e, bg, bu, h);
-                                    else fwd8<3>(r + e, ru + e, bg, bu, h);
-                                    *at = pack8<T>(h);
-                                } else {
-                                    float z[16];
-                                    if (P.act == 0) dz8<T, 0>(r + e, ru + e, bg, bu, *at, z);
-                                    else if (P.act == 1) dz8<T, 1>(r + e, ru + e, bg, bu, *at, z);
-                                    else if (P.act == 2) dz8<T, 2>(r + e, ru + e, bg, bu, *at, z);
-                                    else dz8<T, 3>(r + e, ru + e, bg, bu, *at, z);
-                                    *at = pack8<T>(z);  // dg takes dh's place
-                                    *reinterpret_cast<uint4*>(buf2 + lane * LD * 2 + (s + e) * 2) = pack8<T>(z + 8);
-                                    if (P.db) {
-                                        if (row >= P.M) {  // rows behind the last one add nothing, whatever they hold
+                                if (P.act == 0) fwd8<0>(r + e, ru + e, bg, bu, h);
+                                else if (P.act == 1) fwd8<1>(r + e, ru + e, bg, bu, h);
+                                else if (P.act == 2) fwd8<2>(r + e, ru + e, bg, bu, h);
+                                else fwd8<3>(r + e, ru + e, bg, bu, h);
+                            } else {
 #pragma unroll
-                                            for (int j = 0; j < 16; ++j) z[j] = 0.f;
-                                        }
-                                        const float sum = column_sums(z, lane);
-                                        // one lane of one warp owns each of these sums: the additions keep their order
-                                        const int c = col + s + e + (lane & 7);
-                                        if (lane < 16 && c < P.N)
-                                            atomicAdd(P.db + ((size_t)blockIdx.x * 4 + q) * 2 * P.F + (lane < 8 ? 0 : P.F) + c, sum);
-                                    }
-                                }
+                                for (int j = 0; j < 8; ++j) h[j] = __uint_as_float(r[e + j]);
                             }
-                        } else {
-                            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                            const float* v = reinterpret_cast<const float*>(r);
-                            *reinterpret_cast<uint4*>(mine + s * 2) = pack8<T>(v);
-                            *reinterpret_cast<uint4*>(mine + s * 2 + 16) = pack8<T>(v + 8);
+                            *reinterpret_cast<uint4*>(mine + (s + e) * 2) = pack8<T>(h);
                         }
                     }
                     __syncwarp();
@@ -651,21 +750,48 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
     }
 }
 
-// dW from the partial tiles: tile t is the sum of the slots b + t of the CTAs whose shares of a block's units meet it,
-// in the order of b.  One thread, 4 columns; grid: (rows of a tile) x tiles.
+// db from the CTAs' column sums [rows][n]: 8 columns a block of 256 threads, 32 rows at a time, added in fp64
+__device__ __forceinline__ void db_sum(const float* part, float* db, int rows, int n, int block) {
+    const int x = threadIdx.x & 7, y = threadIdx.x >> 3, col = block * 8 + x;
+    __shared__ double sh[32][9];
+    double s = 0.0;
+    if (col < n)
+#pragma unroll 8
+        for (int r = y; r < rows; r += 32) s += part[(size_t)r * n + col];
+    sh[y][x] = s;
+    __syncthreads();
+    if (threadIdx.x < 8 && col < n) {
+        double v = 0.0;
+        for (int i = 0; i < 32; ++i) v += sh[i][x];
+        db[col] = (float)v;
+    }
+}
+
+// dW from the partial tiles: tile t is the sum of the slots b + t of the groups of CTAs whose shares of a block's units meet
+// it, in the order of b.  One thread, 4 columns; grid: (rows of a tile) x tiles.  Further blocks (blockIdx.y = ntp, or 0
+// where ntp is 0) sum db.
 template <class T, int BN, int CG>
-__global__ void __launch_bounds__(256) k_dw_sum(const float* part, T* dw, int F, int K, int tile0, int ntp, int blk, int ctas,
-                                                int ntn) {
+__global__ void __launch_bounds__(256) k_dw_sum(const float* part, T* dw, int F, int K, int tile0, int ntp, int blk, int groups,
+                                                int ntn, const float* db_part, float* db, int db_rows) {
     constexpr int C4 = BN / 4, R = BM * CG;
-    const int t = blockIdx.y, idx = blockIdx.x * 256 + threadIdx.x, r = idx / C4, c = (idx % C4) * 4;
+    const int t = blockIdx.y;
+    if (t == ntp) {
+        after_previous();
+        for (int b = blockIdx.x; b * 8 < 2 * F; b += gridDim.x) {
+            db_sum(db_part, db, db_rows, 2 * F, b);
+            __syncthreads();
+        }
+        return;
+    }
+    const int idx = blockIdx.x * 256 + threadIdx.x, r = idx / C4, c = (idx % C4) * 4;
     const int tile = tile0 + t, half_tiles = (F + BM - 1) / BM;
     const int mt = (tile / ntn) * CG + r / BM, up = mt >= half_tiles;
     const int f = (up ? mt - half_tiles : mt) * BM + r % BM, k = (tile % ntn) * BN + c;
-    const int U = ntp * blk, lo = t * blk, hi = lo + blk;  // U x ctas stays below 2^31: 148 tiles, 64 chunks, 148 CTAs
-    int b0 = lo * ctas / U, b1 = hi * ctas / U;
-    while (b0 > 0 && U * b0 / ctas > lo) --b0;             // the CTA whose share holds lo ..
-    while (U * (b0 + 1) / ctas <= lo) ++b0;
-    while (b1 >= ctas || U * b1 / ctas >= hi) --b1;        // .. to the one whose share holds hi - 1
+    const int U = ntp * blk, lo = t * blk, hi = lo + blk;  // U x groups stays below 2^31: 148 tiles, 64 chunks, 148 groups
+    int b0 = lo * groups / U, b1 = hi * groups / U;
+    while (b0 > 0 && U * b0 / groups > lo) --b0;           // the group whose share holds lo ..
+    while (U * (b0 + 1) / groups <= lo) ++b0;
+    while (b1 >= groups || U * b1 / groups >= hi) --b1;    // .. to the one whose share holds hi - 1
     after_previous();
     if (f >= F || k >= K) return;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -683,23 +809,6 @@ __global__ void __launch_bounds__(256) k_dw_sum(const float* part, T* dw, int F,
             if constexpr (sizeof(T) == 4) dst[j] = v[j];
             else dst[j] = Half2<T>::one(v[j]);
         }
-}
-
-// db from the CTAs' column sums [rows][n]: 32 columns a block, 32 rows at a time, added in fp64
-__global__ void __launch_bounds__(1024) k_db_sum(const float* part, float* db, int rows, int n) {
-    __shared__ double sh[32][33];
-    const int x = threadIdx.x & 31, y = threadIdx.x >> 5, col = blockIdx.x * 32 + x;
-    double s = 0.0;
-    after_previous();
-    if (col < n)
-#pragma unroll 4
-        for (int r = y; r < rows; r += 32) s += part[(size_t)r * n + col];
-    sh[y][x] = s;
-    __syncthreads();
-    double v = sh[x][y];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (x == 0 && blockIdx.x * 32 + y < n) db[blockIdx.x * 32 + y] = (float)v;
 }
 
 // rows of 16-bit numbers copied to rows of `ldd` (a multiple of 8), zeros behind the n-th; two matrices in one launch
@@ -785,13 +894,13 @@ __global__ void __launch_bounds__(256) k_ff_rows(int M, int K, int F, int act, c
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             if (lane != r || m0 + r >= M) continue;
-            float a, d;
-            const float x = g[r] + bg;
-            if (act == 0) act1<0, false>(x, a, d);
-            else if (act == 1) act1<1, false>(x, a, d);
-            else if (act == 2) act1<2, false>(x, a, d);
-            else act1<3, false>(x, a, d);
-            h[(size_t)(m0 + r) * F + f] = Half2<T>::one(a * (u[r] + bu));
+            f2 a, d;
+            const f2 x = all(g[r] + bg);
+            if (act == 0) act2<0, false>(x, a, d);
+            else if (act == 1) act2<1, false>(x, a, d);
+            else if (act == 2) act2<2, false>(x, a, d);
+            else act2<3, false>(x, a, d);
+            h[(size_t)(m0 + r) * F + f] = Half2<T>::one(un(a).x * (u[r] + bu));
         }
     }
 }
@@ -936,10 +1045,6 @@ static cudaError_t pair_tiles(const Call& c, Args P, int* ctas) {
     P.nk = (c.K + BK - 1) / BK;
     const int groups = (int)std::min<long long>((long long)((c.M + rows - 1) / rows) * ((c.F + tn - 1) / tn), c.nsm / sh.cg);
     *ctas = groups * sh.cg;
-    if (MODE == DZ && P.db) {
-        cudaError_t e = cudaMemsetAsync(P.db, 0, (size_t)*ctas * 4 * 2 * c.F * 4, c.st);
-        if (e != cudaSuccess) return e;
-    }
     if (sh.bn == 64) return launch<T, MODE, 64, 1>(P, groups, c.st);
     if (sh.bn == 128) return launch<T, MODE, 128, 1>(P, groups, c.st);
     return launch<T, MODE, 256, 2>(P, groups, c.st);
@@ -966,7 +1071,7 @@ static cudaError_t forward(Call c, const Plan& L, void* h) {
 }
 
 template <class T, int BN, int CG>
-static cudaError_t dw_passes(const Call& c, const Plan& L, Args P, void* dw, int dw_type) {
+static cudaError_t dw_passes(const Call& c, const Plan& L, Args P, void* dw, int dw_type, const float* db_part, float* db, int db_rows) {
     const int ntn = (c.K + BN - 1) / BN;
     for (int t0 = 0; t0 < L.tiles; t0 += L.ntp) {
         P.tile0 = t0;
@@ -975,11 +1080,13 @@ static cudaError_t dw_passes(const Call& c, const Plan& L, Args P, void* dw, int
         static_assert(148ll * DW_BLOCK * 148 < (1ll << 31), "k_dw_sum's products");
         cudaError_t e = launch<T, DW, BN, CG>(P, groups, c.st);
         if (e != cudaSuccess) return e;
-        const dim3 grid(CG * BM * BN / 4 / 256, P.ntp);
+        const dim3 grid(CG * BM * BN / 4 / 256, P.ntp + (db ? 1 : 0));
         const float* part = (const float*)P.out;
-        e = dw_type == 0
-                ? go(1, k_dw_sum<float, BN, CG>, grid, 256, 0, c.st, part, (float*)dw, c.F, c.K, t0, P.ntp, L.blk, groups, ntn)
-                : go(1, k_dw_sum<T, BN, CG>, grid, 256, 0, c.st, part, (T*)dw, c.F, c.K, t0, P.ntp, L.blk, groups, ntn);
+        e = dw_type == 0 ? go(1, k_dw_sum<float, BN, CG>, grid, 256, 0, c.st, part, (float*)dw, c.F, c.K, t0, P.ntp, L.blk, groups,
+                              ntn, db_part, db, db_rows)
+                         : go(1, k_dw_sum<T, BN, CG>, grid, 256, 0, c.st, part, (T*)dw, c.F, c.K, t0, P.ntp, L.blk, groups, ntn,
+                              db_part, db, db_rows);
+        db = nullptr;  // with the first pass
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
@@ -992,18 +1099,17 @@ static cudaError_t backward(Call c, const Plan& L, const void* dh, void* dx, voi
     const int Fp = pad8(c.F);
     T* z = (T*)(c.ws + L.z);
     const T* Wu = (const T*)c.W + c.F * c.ldw;
+    int ctas;
     {   // z = [dg | du] and the column sums
         Args P = {};
         P.out = z; P.ldo = 2 * Fp;
         P.dh = dh;
         P.vec = c.F % 8 == 0 && ((uintptr_t)dh & 15) == 0;
         P.db = db ? (float*)(c.ws + L.db) : nullptr;
-        int ctas;
         e = pair_tiles<T, DZ>(c, P, &ctas);
-        if (e == cudaSuccess && db)
-            e = go(1, k_db_sum, dim3((2 * c.F + 31) / 32), 1024, 0, c.st, (const float*)P.db, db, ctas * 4, 2 * c.F);
         if (e != cudaSuccess) return e;
     }
+    const float* db_part = (const float*)(c.ws + L.db);
     if (dx) {
         Args P = {};
         if (!map2d(&P.a0, c.type, z, c.F, c.M, 2 * Fp, BM) || !map2d(&P.a1, c.type, z + Fp, c.F, c.M, 2 * Fp, BM) ||
@@ -1029,10 +1135,13 @@ static cudaError_t backward(Call c, const Plan& L, const void* dh, void* dx, voi
         P.M = c.M; P.N = c.K; P.F = c.F;
         P.nk = (c.M + BK - 1) / BK;
         P.out = c.ws + L.part;
-        e = L.dw.bn == 64    ? dw_passes<T, 64, 1>(c, L, P, dw, dw_type)
-            : L.dw.bn == 128 ? dw_passes<T, 128, 1>(c, L, P, dw, dw_type)
-                             : dw_passes<T, 256, 2>(c, L, P, dw, dw_type);
+        return L.dw.bn == 64    ? dw_passes<T, 64, 1>(c, L, P, dw, dw_type, db_part, db, ctas * 4)
+               : L.dw.bn == 128 ? dw_passes<T, 128, 1>(c, L, P, dw, dw_type, db_part, db, ctas * 4)
+                                : dw_passes<T, 256, 2>(c, L, P, dw, dw_type, db_part, db, ctas * 4);
     }
+    if (db)
+        e = go(1, k_dw_sum<T, 64, 1>, dim3((2 * c.F + 7) / 8, 1), 256, 0, c.st, (const float*)nullptr, (T*)nullptr, c.F, c.K, 0, 0, 0, 1,
+               1, db_part, db, ctas * 4);
     return e;
 }
 

@@ -21,9 +21,9 @@
 // the same bits for the same list of lengths on the same kind of card, no counter that a call would have to clear.
 // The second launch walks the chunks backwards: what the first read last is still in L2.
 //
-// Networks up to SMALL_MAX numbers run as one launch of one 16-CTA cluster: the block sums cross in
-// distributed shared memory behind the hardware's cluster barrier, and the parameters and moments are
-// fetched to L2 while the norm is being taken.
+// Networks of up to CL * R chunks of CH_SMALL run as one launch of one 16-CTA cluster: every thread reads its numbers once
+// and holds them in registers, the block sums cross in distributed shared memory behind the hardware's cluster barrier,
+// and the results are written.  REPLACE_SMALL
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -35,9 +35,9 @@ namespace g1opt {
 
 constexpr int THREADS = 256;          // threads a block of the two-launch path
 constexpr int CTAS_PER_SM = 8;
-constexpr int CL = 16, CL_THREADS = 512;  // the cluster of the small path
-constexpr long long SMALL_MAX = 1 << 18;
-constexpr int CH_SMALL = 2048, CH_BIG = 8192;  // numbers a chunk
+constexpr int CL = 16, CL_THREADS = 512, R = 4;  // the small path: CTAs of its cluster, chunks a CTA holds
+constexpr int CH_SMALL = 2048, CH_BIG = 8192;    // numbers a chunk
+static_assert(CH_SMALL == 4 * CL_THREADS, "four numbers a thread");
 constexpr int MAX_PARTS = 2048;
 constexpr int TAB = 48, TAB_BIG = 480;
 
@@ -76,13 +76,27 @@ struct alignas(sizeof(T) * N) Vec {
     T x[N];
 };
 
-__device__ __forceinline__ int find(const Entry* t, int n, long long c) {
-    int lo = 0, hi = n - 1;  // the last entry whose first chunk is <= c; empty tensors are not in the list
+// the last entry whose first chunk is <= c (empty tensors are not in the list).  A table in the kernel's parameters is
+// searched by every thread for itself; one in memory by the block, whose threads look at all entries at once
+__device__ __forceinline__ int find(const Entry* t, int n, long long c, bool in_memory) {
+    if (in_memory) {
+        int at = -1;
+        for (int i = 0; i < n; i += blockDim.x)
+            at += __syncthreads_count(i + threadIdx.x < n && t[min(i + (int)threadIdx.x, n - 1)].chunk0 <= c);
+        return at;
+    }
+    int lo = 0, hi = n - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (t[mid].chunk0 <= c) lo = mid; else hi = mid - 1;
     }
     return lo;
+}
+
+// A launch may start while the one before it in the stream ends: wait here before the first access to memory
+__device__ __forceinline__ void after_previous() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
 }
 
 // numbers before the first 16-byte boundary (element types divide 16)
@@ -195,19 +209,12 @@ __device__ __forceinline__ void advance(const Args& A, const Entry* tab, int fir
     }
 }
 
-__device__ __forceinline__ double norm_chunks(const Args& A, const Entry* tab, int first, int stride, bool prefetch) {
+__device__ __forceinline__ double norm_chunks(const Args& A, const Entry* tab, int first, int stride) {
     double acc = 0.0;
     for (long long c = first; c < A.chunks; c += stride) {
-        const Entry& e = tab[find(tab, A.n, c)];
+        const Entry& e = tab[find(tab, A.n, c, A.table)];
         const long long off = (c - e.chunk0) * A.ch;
         const int cnt = (int)min((long long)A.ch, e.n - off);
-        if (prefetch) {  // one 128-byte line a thread: p, m and v are wanted right after the barrier
-            for (int i = threadIdx.x * 32; i < cnt; i += blockDim.x * 32) {
-                asm volatile("prefetch.global.L2 [%0];" ::"l"(e.p + off + i));
-                asm volatile("prefetch.global.L2 [%0];" ::"l"(e.m + off + i));
-                asm volatile("prefetch.global.L2 [%0];" ::"l"(e.v + off + i));
-            }
-        }
         if (e.type == 0) acc += sumsq((const float*)e.g + off, cnt);
         else if (e.type == 1) acc += sumsq((const __nv_bfloat16*)e.g + off, cnt);
         else acc += sumsq((const __half*)e.g + off, cnt);
@@ -222,18 +229,20 @@ __device__ __forceinline__ float clip_factor(const Args& A, double total, bool w
     return c > 1.0 ? 1.f : (float)c;  // a NaN norm stays NaN, as in torch
 }
 
-__device__ __forceinline__ void apply_chunks(const Args& A, const Entry* tab, float c, int first, int stride) {
+__device__ __forceinline__ Coef coef_of(const Args& A, float c, float lr) {
     Coef k;
-    float lr = 0.f;
-    if (A.adam) {
-        lr = A.lr_dev ? *A.lr_dev : A.lr;
-        k.c = c; k.omb1 = A.omb1; k.b2 = A.b2; k.omb2 = A.omb2; k.eps = A.eps;
-        k.decay = 1.f - lr * A.wd;
-    }
+    k.c = c; k.omb1 = A.omb1; k.b2 = A.b2; k.omb2 = A.omb2; k.eps = A.eps;
+    k.decay = 1.f - lr * A.wd;
+    return k;
+}
+
+__device__ __forceinline__ void apply_chunks(const Args& A, const Entry* tab, float c, int first, int stride) {
+    const float lr = A.adam ? (A.lr_dev ? *A.lr_dev : A.lr) : 0.f;
+    Coef k = coef_of(A, c, lr);
     if (first >= A.chunks) return;
     // the block's chunks, last to first
     for (long long ch = first + (A.chunks - 1 - first) / stride * stride; ch >= 0; ch -= stride) {
-        const int t = find(tab, A.n, ch);
+        const int t = find(tab, A.n, ch, A.table);
         const Entry& e = tab[t];
         const long long off = (ch - e.chunk0) * A.ch;
         const int cnt = (int)min((long long)A.ch, e.n - off);
@@ -253,13 +262,15 @@ __device__ __forceinline__ void apply_chunks(const Args& A, const Entry* tab, fl
 }
 
 __global__ void k_table(const __grid_constant__ Table<TAB_BIG> T, int count, Entry* dst) {
+    after_previous();
     for (int i = threadIdx.x; i < count; i += blockDim.x) dst[i] = T.e[i];
 }
 
 __global__ void __launch_bounds__(THREADS) k_norm(const __grid_constant__ Args A, const __grid_constant__ Table<TAB> T) {
     __shared__ double sh[33];
     const Entry* tab = A.table ? A.table : T.e;
-    const double s = block_sum(norm_chunks(A, tab, blockIdx.x, gridDim.x, false), sh);
+    after_previous();
+    const double s = block_sum(norm_chunks(A, tab, blockIdx.x, gridDim.x), sh);
     if (threadIdx.x == 0) A.part[blockIdx.x] = s;
     if (A.adam) advance(A, tab, blockIdx.x * THREADS + threadIdx.x, gridDim.x * THREADS);
 }
@@ -267,25 +278,88 @@ __global__ void __launch_bounds__(THREADS) k_norm(const __grid_constant__ Args A
 __global__ void __launch_bounds__(THREADS) k_apply(const __grid_constant__ Args A, const __grid_constant__ Table<TAB> T) {
     __shared__ double sh[33];
     const Entry* tab = A.table ? A.table : T.e;
+    after_previous();
     double x = 0.0;
+#pragma unroll 4
     for (int i = threadIdx.x; i < A.nparts; i += THREADS) x += A.part[i];
     const double total = block_sum(x, sh);
     const float c = clip_factor(A, total, blockIdx.x == 0 && threadIdx.x == 0);
     apply_chunks(A, tab, c, blockIdx.x, gridDim.x);
 }
 
+// four neighbours of a tensor, the first `cnt` of them inside it; a wide access where the address and cnt allow it
+template <class T>
+__device__ __forceinline__ void load4(const T* p, int cnt, float* x) {
+    if (cnt >= 4 && ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0) {
+        const Vec<T, 4> v = *reinterpret_cast<const Vec<T, 4>*>(p);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = to_f(v.x[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = k < cnt ? to_f(p[k]) : 0.f;
+    }
+}
+template <class T>
+__device__ __forceinline__ void store4(T* p, int cnt, const float* x) {
+    if (cnt >= 4 && ((uintptr_t)p & (4 * sizeof(T) - 1)) == 0) {
+        Vec<T, 4> v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) from_f(x[k], v.x[k]);
+        *reinterpret_cast<Vec<T, 4>*>(p) = v;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (k < cnt) from_f(x[k], p[k]);
+    }
+}
+
+template <bool ADAM>
 __global__ void __launch_bounds__(CL_THREADS) k_small(const __grid_constant__ Args A, const __grid_constant__ Table<TAB> T) {
     __shared__ double sh[33];
     __shared__ double mine;
+    __shared__ int s_at[R];
     const Entry* tab = A.table ? A.table : T.e;
-    const int r = blockIdx.x;  // the grid is one cluster
-    const double s = block_sum(norm_chunks(A, tab, r, CL, A.adam != 0), sh);
-    if (threadIdx.x == 0) mine = s;
-    if (A.adam) advance(A, tab, r * CL_THREADS + (CL_THREADS - 1 - threadIdx.x), CL * CL_THREADS);
+    const int r = blockIdx.x, tid = threadIdx.x;  // the grid is one cluster
+    after_previous();
+    if (A.table) {
+        for (int j = 0; j < R; ++j) {
+            const int at = find(tab, A.n, r + j * CL, true);
+            if (tid == 0) s_at[j] = at;
+        }
+    } else if (tid < R) {
+        s_at[tid] = find(tab, A.n, r + tid * CL, false);
+    }
+    __syncthreads();
+    float g[R][4], p[ADAM ? R : 1][4], m[ADAM ? R : 1][4], v[ADAM ? R : 1][4];
+    long long off[R];
+    int cnt[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        const Entry& e = tab[max(s_at[j], 0)];
+        off[j] = (r + j * CL - e.chunk0) * CH_SMALL + 4 * tid;
+        cnt[j] = r + j * CL < A.chunks ? (int)min(4ll, max(0ll, e.n - off[j])) : 0;
+        if (e.type == 0) load4((const float*)e.g + off[j], cnt[j], g[j]);
+        else if (e.type == 1) load4((const __nv_bfloat16*)e.g + off[j], cnt[j], g[j]);
+        else load4((const __half*)e.g + off[j], cnt[j], g[j]);
+        if (ADAM) {
+            load4(e.p + off[j], cnt[j], p[ADAM ? j : 0]);
+            load4(e.m + off[j], cnt[j], m[ADAM ? j : 0]);
+            load4(e.v + off[j], cnt[j], v[ADAM ? j : 0]);
+        }
+    }
+    if (ADAM) advance(A, tab, r * CL_THREADS + (CL_THREADS - 1 - tid), CL * CL_THREADS);
+    double acc = 0.0;
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) { const double x = g[j][k]; acc = fma(x, x, acc); }
+    const double s = block_sum(acc, sh);
+    if (tid == 0) mine = s;
     __syncthreads();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     double total = 0.0;
+#pragma unroll
     for (int k = 0; k < CL; ++k) {
         uint32_t a = (uint32_t)__cvta_generic_to_shared(&mine), remote;
         double x;
@@ -295,19 +369,56 @@ __global__ void __launch_bounds__(CL_THREADS) k_small(const __grid_constant__ Ar
     }
     // no CTA leaves before the others have read its sum
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    const float c = clip_factor(A, total, r == 0 && threadIdx.x == 0);
-    apply_chunks(A, tab, c, r, CL);
+    const float c = clip_factor(A, total, r == 0 && tid == 0);
+    const float lr = ADAM ? (A.lr_dev ? *A.lr_dev : A.lr) : 0.f;
+    Coef k = coef_of(A, c, lr);
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        const Entry& e = tab[max(s_at[j], 0)];
+        if (cnt[j] == 0) continue;
+        if constexpr (ADAM) {
+            const float2 b = A.bias[max(s_at[j], 0)];
+            k.a = lr * b.x;
+            k.rb2 = b.y;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) adam1(g[j][i], p[j][i], m[j][i], v[j][i], k);
+            store4(e.p + off[j], cnt[j], p[j]);
+            store4(e.m + off[j], cnt[j], m[j]);
+            store4(e.v + off[j], cnt[j], v[j]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) g[j][i] *= c;
+            if (e.type == 0) store4((float*)e.g + off[j], cnt[j], g[j]);
+            else if (e.type == 1) store4((__nv_bfloat16*)e.g + off[j], cnt[j], g[j]);
+            else store4((__half*)e.g + off[j], cnt[j], g[j]);
+        }
+    }
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// a launch that may start while its predecessor in the stream ends (after_previous), in clusters of `cl` CTAs
+template <class... P, class... A>
+static cudaError_t go(int cl, void (*k)(P...), int grid, int block, cudaStream_t st, const A&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid; cfg.blockDim = block; cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cl; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = cl > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, k, args...);
+}
+
 // whether a 16-CTA cluster of k_small fits on the current device (asked once a device)
+template <bool ADAM>
 static bool cluster_fits(int dev) {
     static std::once_flag once[64];
     static bool ok[64];
     if (dev < 0 || dev >= 64) return false;
     std::call_once(once[dev], [dev]() {
         ok[dev] = false;
-        if (cudaFuncSetAttribute(k_small, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return;
+        if (cudaFuncSetAttribute(k_small<ADAM>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = CL; cfg.blockDim = CL_THREADS;
         cudaLaunchAttribute at[1];
@@ -315,7 +426,7 @@ static bool cluster_fits(int dev) {
         at[0].val.clusterDim.x = CL; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
         cfg.attrs = at; cfg.numAttrs = 1;
         int n = 0;
-        ok[dev] = cudaOccupancyMaxActiveClusters(&n, k_small, &cfg) == cudaSuccess && n >= 1;
+        ok[dev] = cudaOccupancyMaxActiveClusters(&n, k_small<ADAM>, &cfg) == cudaSuccess && n >= 1;
         (void)cudaGetLastError();
     });
     return ok[dev];
@@ -372,11 +483,11 @@ static int run(const char* who, int n, void* const* g, const int* types, float* 
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&nsm, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) { set_error((int)e, who, cudaGetErrorString(e)); return -1; }
-    const bool small = total <= SMALL_MAX && cluster_fits(dev);
     // short chunks while there are too few long ones to give every resident block two
     A.ch = total <= 2ll * nsm * CTAS_PER_SM * CH_BIG ? CH_SMALL : CH_BIG;
     long long c0 = 0;
     for (Entry& q : tab) { q.chunk0 = c0; c0 += (q.n + A.ch - 1) / A.ch; }
+    const bool small = A.ch == CH_SMALL && c0 <= CL * R && (A.adam ? cluster_fits<true>(dev) : cluster_fits<false>(dev));
     A.chunks = c0;
     A.n = (int)tab.size();
     A.steps = steps;
@@ -392,24 +503,18 @@ static int run(const char* who, int n, void* const* g, const int* types, float* 
         for (int i = 0; i < A.n; i += TAB_BIG) {
             const int cnt = std::min(TAB_BIG, A.n - i);
             for (int k = 0; k < cnt; ++k) B.e[k] = tab[i + k];
-            k_table<<<1, 256, 0, st>>>(B, cnt, dst + i);
+            e = go(1, k_table, 1, 256, st, B, cnt, dst + i);
+            if (e != cudaSuccess) break;
         }
         A.table = dst;
     }
-    if (small) {
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = CL; cfg.blockDim = CL_THREADS; cfg.stream = st;
-        cudaLaunchAttribute at[1];
-        at[0].id = cudaLaunchAttributeClusterDimension;
-        at[0].val.clusterDim.x = CL; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-        cfg.attrs = at; cfg.numAttrs = 1;
-        e = cudaLaunchKernelEx(&cfg, k_small, A, T);
-    } else {
+    if (e == cudaSuccess && small) {
+        e = A.adam ? go(CL, k_small<true>, CL, CL_THREADS, st, A, T) : go(CL, k_small<false>, CL, CL_THREADS, st, A, T);
+    } else if (e == cudaSuccess) {
         const int grid = (int)std::max(1ll, std::min<long long>(A.chunks, std::min(nsm * CTAS_PER_SM, MAX_PARTS)));
         A.nparts = grid;
-        k_norm<<<grid, THREADS, 0, st>>>(A, T);
-        k_apply<<<grid, THREADS, 0, st>>>(A, T);
-        e = cudaGetLastError();
+        e = go(1, k_norm, grid, THREADS, st, A, T);
+        if (e == cudaSuccess) e = go(1, k_apply, grid, THREADS, st, A, T);
     }
     if (e != cudaSuccess) { set_error((int)e, who, cudaGetErrorString(e)); return -1; }
     return 0;

@@ -303,7 +303,7 @@ def _on(dev):
 
 def _stream_of(dev):
     """torch's current stream on `dev`, as the number that the C-ABI takes"""
-    return torch.cuda.current_stream(dev).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def _rows(t):
@@ -389,15 +389,19 @@ def gated_ff_backward_device(dh, x, w, b=None, act="silu", need=(True, True, Tru
         raise G1Error("dw is fp32 or of the rows' type")
     if dh.device != dev or dh.dtype != x.dtype or dh.shape != x.shape[:-1] + (F,):
         raise G1Error("dh must be [..., F] on x's device and of its type")
-    dh = dh.contiguous()
     with _on(dev):
-        M, K, px, ldx, pw, ldw, n, ws = _ff_ws(lib, x2, w, F, 1)
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need[0] else None
-        dw = torch.empty(2 * F, K, dtype=dw_dtype, device=dev) if need[1] else None
-        db = torch.empty(2 * F, dtype=torch.float32, device=dev) if need[2] else None
-        if lib.g1_gated_ff_backward(M, K, F, t, code, dh.data_ptr(), px, ldx, pw, ldw, _addr(b), _addr(dx), _addr(dw),
-                                    _FF_TYPE.get(dw_dtype, 0), _addr(db), _addr(ws), n, _stream_of(dev)):
-            _check()
+        return _ff_backward(lib, dev, dh, x.shape, F, t, code, b, _ff_ws(lib, x2, w, F, 1), need, x.dtype, dw_dtype)
+
+
+def _ff_backward(lib, dev, dh, x_shape, F, t, code, b, operands, need, dtype, dw_dtype):
+    M, K, px, ldx, pw, ldw, n, ws = operands
+    dh = dh.contiguous()
+    dx = torch.empty(x_shape, dtype=dtype, device=dev) if need[0] else None
+    dw = torch.empty(2 * F, K, dtype=dw_dtype, device=dev) if need[1] else None
+    db = torch.empty(2 * F, dtype=torch.float32, device=dev) if need[2] else None
+    if lib.g1_gated_ff_backward(M, K, F, t, code, dh.data_ptr(), px, ldx, pw, ldw, _addr(b), _addr(dx), _addr(dw),
+                                _FF_TYPE.get(dw_dtype, 0), _addr(db), _addr(ws), n, _stream_of(dev)):
+        _check()
     return dx, dw, db
 
 
@@ -409,18 +413,38 @@ def gated_ff_status():
 class _GatedFF(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, act):
+        lib = load_library()
         w16 = w if w.dtype == x.dtype else w.to(x.dtype)
-        ctx.save_for_backward(x, w16, b)
-        ctx.act, ctx.w_dtype = act, w.dtype
-        return gated_ff_device(x, w16, b, act)
+        x2, w2, b2, t, code = _ff_args(x, w16, b, act)
+        F, dev = w2.shape[0] // 2, x2.device
+        with _on(dev):
+            M, K, px, ldx, pw, ldw, n, ws = _ff_ws(lib, x2, w2, F, 0)
+            h = torch.empty(x.shape[:-1] + (F,), dtype=x.dtype, device=dev)
+            if lib.g1_gated_ff(M, K, F, t, code, px, ldx, pw, ldw, _addr(b2), h.data_ptr(), _addr(ws), n, _stream_of(dev)):
+                _check()
+        if n and M > 4:  # the backward pass takes the copies with aligned rows that this call left in ws
+            at, k8 = ws.data_ptr(), (K + 7) & ~7
+            if px & 15 or ldx & 7:
+                px, ldx = at, k8
+                at += (M * k8 * 2 + 255) & ~255
+            if pw & 15 or ldw & 7:
+                pw, ldw = at, k8
+        ctx.save_for_backward(x, w if w16 is w else w16, b)
+        ctx.call = (lib, dev, F, t, code, M, K, px, ldx, pw, ldw, w.dtype)
+        ctx.keep = (x2, w2, b2, ws)
+        return h
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
-        x, w16, b = ctx.saved_tensors
-        need = (ctx.needs_input_grad[0], ctx.needs_input_grad[1], b is not None and ctx.needs_input_grad[2])
-        dx, dw, db = gated_ff_backward_device(dh, x, w16, b, ctx.act, need, ctx.w_dtype)
-        return dx, dw, db if db is None else db.to(b.dtype), None
+        x, w, b = ctx.saved_tensors  # notices a change made since
+        lib, dev, F, t, code, M, K, px, ldx, pw, ldw, w_dtype = ctx.call
+        need = ctx.needs_input_grad
+        with _on(dev):
+            n = lib.g1_gated_ff_workspace(M, K, F, px, ldx, pw, ldw, 1)
+            ops = (M, K, px, ldx, pw, ldw, n, torch.empty(n, dtype=torch.uint8, device=dev))
+            dx, dw, db = _ff_backward(lib, dev, dh, x.shape, F, t, code, ctx.keep[2], ops, need, x.dtype, w_dtype)
+        return dx, dw, db if db is None or b.dtype == torch.float32 else db.to(b.dtype), None
 
 
 def gated_ff(x, w, b=None, act="silu"):
@@ -515,24 +539,28 @@ def _dense(t):
     return t.permute(order).is_contiguous()
 
 
-def _cuda_list(tensors, what, types):
-    dev = None
+def _cuda_list(tensors, what, types, dev=None):
+    """The device of a list of dense CUDA tensors of those types (dev where that is the one it must be)."""
     for t in tensors:
-        if not t.is_cuda:
-            raise G1Error(f"{what} must be CUDA tensors")
         if dev is None:
             dev = t.device
+        if not t.is_cuda:
+            raise G1Error(f"{what} must be CUDA tensors")
         if t.device != dev:
             raise G1Error(f"{what} must be on one device")
         if t.dtype not in types:
             raise G1Error(f"{what} must be {' / '.join(str(x)[6:] for x in types)}, not {str(t.dtype)[6:]}")
-        if not _dense(t):
+        if not t.is_contiguous() and not _dense(t):
             raise G1Error(f"{what} must fill their memory without gaps (use .contiguous())")
     return dev
 
 
+def _array(ctype, values):
+    return (ctype * len(values))(*values)
+
+
 def _ptrs(tensors):
-    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+    return _array(ctypes.c_void_p, [t.data_ptr() for t in tensors])
 
 
 def clip_grad_norm_device(grads, max_norm):
@@ -541,20 +569,20 @@ def clip_grad_norm_device(grads, max_norm):
     current stream.  Returns the norm before clipping as a CUDA fp32 scalar; nothing synchronises.  The
     squares are summed in fp64 in a fixed order.  A norm that is NaN or infinite scales as in
     torch.nn.utils.clip_grad_norm_.  Tensors of one call may not share memory."""
-    _require_gpu()
     lib = load_library()
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     dev = _cuda_list(grads, "gradients", _GRAD_TYPE)
     if dev is None:
+        _require_gpu()
         dev = torch.device("cuda", torch.cuda.current_device())
     n = len(grads)
     norm = torch.empty((), dtype=torch.float32, device=dev)
     size = lib.g1_opt_workspace(n)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
     with _on(dev):
-        rc = lib.g1_clip_grad_norm(n, _ptrs(grads), (ctypes.c_int * n)(*[_GRAD_TYPE[g.dtype] for g in grads]),
-                                   (ctypes.c_longlong * n)(*[g.numel() for g in grads]), float(max_norm), _dp(norm),
-                                   _dp(ws), size, _stream())
+        rc = lib.g1_clip_grad_norm(n, _ptrs(grads), _array(ctypes.c_int, [_GRAD_TYPE[g.dtype] for g in grads]),
+                                   _array(ctypes.c_longlong, [g.numel() for g in grads]), max_norm, norm.data_ptr(),
+                                   ws.data_ptr(), size, _stream_of(dev))
     if rc:
         _check()
     torch.autograd.graph.increment_version(grads)
@@ -595,6 +623,9 @@ class ClipAdam:
                 if m.shape != p.shape or m.stride() != p.stride():
                     raise G1Error("moments must be laid out like their parameters")
         self.steps = torch.full((len(self.params),), int(steps), dtype=torch.int64, device=self.device)
+        self._counts = [p.numel() for p in self.params]
+        self._strides = [p.stride() for p in self.params]
+        self._state = self.exp_avg + self.exp_avg_sq + [self.steps]
 
     def zero_grad(self, set_to_none=True):
         for p in self.params:
@@ -603,44 +634,44 @@ class ClipAdam:
             elif p.grad is not None:
                 p.grad.zero_()
 
-    @torch.no_grad()
     def step(self, grads=None):
-        params, n = self.params, len(self.params)
+        params, n, dev = self.params, len(self.params), self.device
         grads = [p.grad for p in params] if grads is None else list(grads)
         if len(grads) != n:
             raise G1Error("step takes one gradient (or None) a parameter")
-        for i, (g, p) in enumerate(zip(grads, params)):
+        lib = _lib
+        ptrs, types, counts, moved = [None] * n, [0] * n, [0] * n, []
+        for i, g in enumerate(grads):
             if g is None:
                 continue
+            p = params[i]
             if g.shape != p.shape:
                 raise G1Error("gradients must have their parameters' shapes")
-            if g.stride() != p.stride() and g.numel():
-                if not g.is_cuda:
-                    raise G1Error("gradients must be CUDA tensors")
-                grads[i] = torch.empty_like(p, dtype=g.dtype).copy_(g)
-        have = [g for g in grads if g is not None]
-        _cuda_list(have + params[:1], "gradients", _GRAD_TYPE)
-        lib, dev = _lib, self.device
+            t = _GRAD_TYPE.get(g.dtype)
+            if t is None or g.device != dev:
+                raise G1Error("gradients must be fp32, bf16 or fp16 on their parameters' device")
+            if p.stride() != self._strides[i] or p.device != dev or p.dtype != torch.float32:
+                raise G1Error("a parameter is no longer laid out as it was when the optimiser was made")
+            if g.stride() != self._strides[i]:
+                g = grads[i] = torch.empty_like(p, dtype=g.dtype, requires_grad=False).copy_(g.detach())
+            ptrs[i], types[i], counts[i] = g.data_ptr(), t, self._counts[i]
+            moved.append(p)
         norm = torch.empty((), dtype=torch.float32, device=dev)
         size = lib.g1_opt_workspace(n)
         ws = torch.empty(size, dtype=torch.uint8, device=dev)
-        lr_dev = None
-        if isinstance(self.lr, torch.Tensor):
-            if not (self.lr.device == dev and self.lr.dtype == torch.float32 and self.lr.numel() == 1):
+        lr, lr_dev = self.lr, None
+        if isinstance(lr, torch.Tensor):
+            if not (lr.device == dev and lr.dtype == torch.float32 and lr.numel() == 1):
                 raise G1Error("a tensor lr must be one fp32 number on the parameters' device")
-            lr_dev = self.lr
-        gp = (ctypes.c_void_p * n)(*[None if g is None else g.data_ptr() for g in grads])
-        types = (ctypes.c_int * n)(*[0 if g is None else _GRAD_TYPE[g.dtype] for g in grads])
-        counts = (ctypes.c_longlong * n)(*[0 if g is None else g.numel() for g in grads])
+            lr, lr_dev = 0.0, lr.data_ptr()
         with _on(dev):
-            rc = lib.g1_clip_adam(n, gp, types, _ptrs(params), _ptrs(self.exp_avg), _ptrs(self.exp_avg_sq), counts,
-                                  _dp(self.steps), self.max_norm, 0.0 if lr_dev is not None else float(self.lr),
-                                  _dp(lr_dev), self.betas[0], self.betas[1], self.eps, self.weight_decay, _dp(norm),
-                                  _dp(ws), size, _stream())
+            rc = lib.g1_clip_adam(n, _array(ctypes.c_void_p, ptrs), _array(ctypes.c_int, types), _ptrs(params),
+                                  _ptrs(self.exp_avg), _ptrs(self.exp_avg_sq), _array(ctypes.c_longlong, counts),
+                                  self.steps.data_ptr(), self.max_norm, lr, lr_dev, self.betas[0], self.betas[1], self.eps,
+                                  self.weight_decay, norm.data_ptr(), ws.data_ptr(), size, _stream_of(dev))
         if rc:
             _check()
-        torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None]
-                                               + self.exp_avg + self.exp_avg_sq + [self.steps])
+        torch.autograd.graph.increment_version(moved + self._state)
         return norm
 
     def state_dict(self):

@@ -182,8 +182,10 @@ int g1_runnorm_update(int dim, float* mean, float* var, double count, const doub
  *   g1_gated_ff_backward  from dh [M][F]: dx [M][K], dw [2F][K] (dw_type 0 fp32, or the inputs' type), db fp32
  *                         [2F]; any of the three may be NULL.  g and u are computed again from X; dg and du are rounded
  *                         to the inputs' type before their products (not in db).  Same inputs, same bits.
- * ws: DEVICE workspace of g1_gated_ff_workspace(...) bytes, 256-byte aligned, for this call alone until it has run (it
- * also holds copies of X and W where their rows do not start on 16-byte boundaries).
+ * ws: DEVICE workspace of g1_gated_ff_workspace(...) bytes, 256-byte aligned, for this call alone until it has run.
+ * Where rows of X (if M > 4 or backward) or of W do not start on 16-byte boundaries, copies whose rows do (stride K
+ * rounded up to 8) are made in it first: X's at its start, W's on the next 256-byte boundary.  A backward call
+ * may be given the copies that its forward call left.
  *   g1_gated_ff_status    nonzero if a wait of these kernels ran out on the current device since the last call
  *                         (synchronous; clears) */
 long long g1_gated_ff_workspace(int M, int K, int F, const void* X, long long ldx, const void* W, long long ldw,
