@@ -12,18 +12,28 @@
 // read twice.  The squares are summed in fp64: an fp32 square overflows from 1.8e19 and vanishes below 1e-23, and
 // a sum of 10^8 of them loses digits; the conversions stay below the time of the loads.
 //
-// A tensor is cut into chunks; a block walks chunks of the whole list (binary search for the chunk's tensor), so
-// one launch serves any number of tensors.  Up to TAB tensors travel in the kernel's parameters; longer lists are
-// laid into the workspace by k_table, whose parameters carry TAB_BIG entries a launch.  Parameters are copied at
-// launch or capture, so a captured call holds no host memory.
+// A tensor is cut into chunks, and a chunk's tensor is found by a search in the list, so one launch serves any number of
+// tensors.  Up to TAB tensors travel in the kernel's parameters; longer lists are laid into the workspace by k_table,
+// whose parameters carry TAB_BIG entries a launch.  Parameters are copied at launch or capture, so a captured call
+// holds no host memory.
 //
-// Block sums go to the workspace and every block of the second launch adds them up in the same order: no atomics,
-// the same bits for the same list of lengths on the same kind of card, no counter that a call would have to clear.
-// The second launch walks the chunks backwards: what the first read last is still in L2.
+// k_norm's block sums go to the workspace and are added up in one order (by every block of k_apply, or once by k_total where
+// k_apply has more blocks than fit): no atomics, the same bits for the same list of lengths and alignments on the same kind
+// of card, no counter that a call would have to clear.  k_apply takes the last chunk first: what k_norm read last is
+// still in L2.
 //
-// Networks of up to CL * R chunks of CH_SMALL run as one launch of one 16-CTA cluster: every thread reads its numbers once
-// and holds them in registers, the block sums cross in distributed shared memory behind the hardware's cluster barrier,
-// and the results are written.  REPLACE_SMALL
+// Networks of up to CL * R chunks of CH_SMALL run as one launch of one 16-CTA cluster (k_small): every thread reads its
+// numbers once and holds them in registers, the block sums cross in distributed shared memory behind the hardware's
+// cluster barrier, and the results are written.
+//
+// Measured on one B200, replayed from a graph (floor: the bytes at the measured 6552 GB/s; memory of the smaller ones stays
+// in L2 between replays):
+//   clip   99387 fp32 in 9 tensors      7 us (12.4 when each chunk was loaded for the norm and again for the clip)
+//          3e6 bf16 in 300 tensors     14 us; floor 1.8
+//          2.7e8 fp32 in 40 tensors   496 us; floor 328, 491 with the second read that 1 GB needs
+//   Adam   99387                       11 us
+//          2270267 in 17 tensors       15 us; floor 9.7
+//          6.7e7, bf16 gradients      305 us; floor 266, 287 with the second read
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -34,18 +44,22 @@
 namespace g1opt {
 
 constexpr int THREADS = 256;          // threads a block of the two-launch path
-constexpr int CTAS_PER_SM = 8;
+// resident blocks an SM that k_norm and k_apply are compiled for: what bounds them is the loads in flight (with the
+// registers that the compiler took, 48 a thread, clipping 2.7e8 numbers took 605 us, with these 496)
+constexpr int NORM_CTAS = 4, ADAM_CTAS = 3, CLIP_CTAS = 6;
+constexpr int UNROLL = 4;
 constexpr int CL = 16, CL_THREADS = 512, R = 4;  // the small path: CTAs of its cluster, chunks a CTA holds
 constexpr int CH_SMALL = 2048, CH_BIG = 8192;    // numbers a chunk
 static_assert(CH_SMALL == 4 * CL_THREADS, "four numbers a thread");
 constexpr int MAX_PARTS = 2048;
-constexpr int TAB = 48, TAB_BIG = 480;
+constexpr int TAB = 48, TAB_BIG = 448;
 
 struct Entry {
     void* g;
     float *p, *m, *v;
     long long n, chunk0;  // numbers; index of the tensor's first chunk
     int type, index;      // 0 fp32, 1 bf16, 2 fp16; place in the caller's list
+    int head, pad;        // numbers before the first 128-byte boundary (of g, of p for Adam): part of the first chunk
 };
 template <int N>
 struct Table {
@@ -93,17 +107,25 @@ __device__ __forceinline__ int find(const Entry* t, int n, long long c, bool in_
     return lo;
 }
 
+// numbers [lo, lo + cnt) of a tensor's chunk: from the second on chunks start on 128-byte boundaries, so that only a
+// tensor's ends take accesses of single numbers (with chunks cut anywhere each one waited for its first few numbers
+// before the rest: clipping 2.7e8 of them took 763 instead of 627 us)
+__device__ __forceinline__ long long chunk_of(const Entry& e, long long c, int ch, int& cnt) {
+    const long long j = c - e.chunk0, lo = j ? e.head + j * ch : 0, hi = min(e.n, e.head + (j + 1) * ch);
+    cnt = (int)(hi - lo);
+    return lo;
+}
+
 // A launch may start while the one before it in the stream ends: wait here before the first access to memory
 __device__ __forceinline__ void after_previous() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
 }
 
-// numbers before the first 16-byte boundary (element types divide 16)
+// numbers before the first 128-byte boundary: from there a warp's accesses are whole lines
 template <class T>
 __device__ __forceinline__ int head_of(const T* p, int cnt) {
-    const int mis = (int)((uintptr_t)p & 15);
-    const int h = mis ? (16 - mis) / (int)sizeof(T) : 0;
+    const int h = (int)(-(uintptr_t)p & 127) / (int)sizeof(T);
     return h < cnt ? h : cnt;
 }
 
@@ -116,7 +138,7 @@ __device__ __forceinline__ double sumsq(const T* p, int cnt) {
     if (tid < head) { const double x = to_f(p[tid]); acc += x * x; }
     if (tid < cnt - tail) { const double x = to_f(p[tail + tid]); acc += x * x; }
     const Vec<T, N>* q = reinterpret_cast<const Vec<T, N>*>(p + head);
-#pragma unroll 4
+#pragma unroll UNROLL
     for (int i = tid; i < nv; i += nt) {
         const Vec<T, N> w = q[i];
 #pragma unroll
@@ -133,7 +155,7 @@ __device__ __forceinline__ void scale(T* p, int cnt, float c) {
     if (tid < head) from_f(to_f(p[tid]) * c, p[tid]);
     if (tid < cnt - tail) from_f(to_f(p[tail + tid]) * c, p[tail + tid]);
     Vec<T, N>* q = reinterpret_cast<Vec<T, N>*>(p + head);
-#pragma unroll 4
+#pragma unroll UNROLL
     for (int i = tid; i < nv; i += nt) {
         Vec<T, N> w = q[i];
 #pragma unroll
@@ -209,12 +231,14 @@ __device__ __forceinline__ void advance(const Args& A, const Entry* tab, int fir
     }
 }
 
-__device__ __forceinline__ double norm_chunks(const Args& A, const Entry* tab, int first, int stride) {
+// the blocks take the chunks in turn, so that all of them read one stretch of memory at a time (runs of neighbours a block
+// need one search only, but measured 756 us where this takes 698: 2.7e8 fp32 numbers, norm and clip)
+__device__ __forceinline__ double norm_chunks(const Args& A, const Entry* tab) {
     double acc = 0.0;
-    for (long long c = first; c < A.chunks; c += stride) {
+    for (long long c = blockIdx.x; c < A.chunks; c += gridDim.x) {
         const Entry& e = tab[find(tab, A.n, c, A.table)];
-        const long long off = (c - e.chunk0) * A.ch;
-        const int cnt = (int)min((long long)A.ch, e.n - off);
+        int cnt;
+        const long long off = chunk_of(e, c, A.ch, cnt);
         if (e.type == 0) acc += sumsq((const float*)e.g + off, cnt);
         else if (e.type == 1) acc += sumsq((const __nv_bfloat16*)e.g + off, cnt);
         else acc += sumsq((const __half*)e.g + off, cnt);
@@ -236,55 +260,75 @@ __device__ __forceinline__ Coef coef_of(const Args& A, float c, float lr) {
     return k;
 }
 
-__device__ __forceinline__ void apply_chunks(const Args& A, const Entry* tab, float c, int first, int stride) {
-    const float lr = A.adam ? (A.lr_dev ? *A.lr_dev : A.lr) : 0.f;
-    Coef k = coef_of(A, c, lr);
-    if (first >= A.chunks) return;
-    // the block's chunks, last to first
-    for (long long ch = first + (A.chunks - 1 - first) / stride * stride; ch >= 0; ch -= stride) {
-        const int t = find(tab, A.n, ch, A.table);
-        const Entry& e = tab[t];
-        const long long off = (ch - e.chunk0) * A.ch;
-        const int cnt = (int)min((long long)A.ch, e.n - off);
-        if (A.adam) {
-            const float2 b = A.bias[t];
-            k.a = lr * b.x;
-            k.rb2 = b.y;
-            if (e.type == 0) adam((const float*)e.g + off, e.p + off, e.m + off, e.v + off, cnt, k);
-            else if (e.type == 1) adam((const __nv_bfloat16*)e.g + off, e.p + off, e.m + off, e.v + off, cnt, k);
-            else adam((const __half*)e.g + off, e.p + off, e.m + off, e.v + off, cnt, k);
-        } else {
-            if (e.type == 0) scale((float*)e.g + off, cnt, c);
-            else if (e.type == 1) scale((__nv_bfloat16*)e.g + off, cnt, c);
-            else scale((__half*)e.g + off, cnt, c);
-        }
+template <bool ADAM>
+__device__ __forceinline__ void apply_chunk(const Args& A, const Entry* tab, float c, long long ch) {
+    const float lr = ADAM ? (A.lr_dev ? *A.lr_dev : A.lr) : 0.f;
+    const int t = find(tab, A.n, ch, A.table);
+    const Entry& e = tab[t];
+    int cnt;
+    const long long off = chunk_of(e, ch, A.ch, cnt);
+    if (ADAM) {
+        Coef k = coef_of(A, c, lr);
+        const float2 b = A.bias[t];
+        k.a = lr * b.x;
+        k.rb2 = b.y;
+        if (e.type == 0) adam((const float*)e.g + off, e.p + off, e.m + off, e.v + off, cnt, k);
+        else if (e.type == 1) adam((const __nv_bfloat16*)e.g + off, e.p + off, e.m + off, e.v + off, cnt, k);
+        else adam((const __half*)e.g + off, e.p + off, e.m + off, e.v + off, cnt, k);
+    } else {
+        if (e.type == 0) scale((float*)e.g + off, cnt, c);
+        else if (e.type == 1) scale((__nv_bfloat16*)e.g + off, cnt, c);
+        else scale((__half*)e.g + off, cnt, c);
     }
 }
 
+// 16 entries a block (one reading them all takes 10 us: each lane of a warp wants other words of the parameters, which
+// come one at a time)
 __global__ void k_table(const __grid_constant__ Table<TAB_BIG> T, int count, Entry* dst) {
+    static_assert(sizeof(Entry) % 8 == 0, "words of 8 bytes");
     after_previous();
-    for (int i = threadIdx.x; i < count; i += blockDim.x) dst[i] = T.e[i];
+    constexpr int W = sizeof(Entry) / 8;
+    const unsigned long long* src = reinterpret_cast<const unsigned long long*>(T.e);
+    const int lo = blockIdx.x * 16 * W, hi = min(lo + 16 * W, count * W);
+    for (int i = lo + threadIdx.x; i < hi; i += 32) reinterpret_cast<unsigned long long*>(dst)[i] = src[i];
 }
 
-__global__ void __launch_bounds__(THREADS) k_norm(const __grid_constant__ Args A, const __grid_constant__ Table<TAB> T) {
+__global__ void __launch_bounds__(THREADS, NORM_CTAS) k_norm(const __grid_constant__ Args A, const __grid_constant__ Table<TAB> T) {
     __shared__ double sh[33];
     const Entry* tab = A.table ? A.table : T.e;
     after_previous();
-    const double s = block_sum(norm_chunks(A, tab, blockIdx.x, gridDim.x), sh);
+    const double s = block_sum(norm_chunks(A, tab), sh);
     if (threadIdx.x == 0) A.part[blockIdx.x] = s;
     if (A.adam) advance(A, tab, blockIdx.x * THREADS + threadIdx.x, gridDim.x * THREADS);
 }
 
-__global__ void __launch_bounds__(THREADS) k_apply(const __grid_constant__ Args A, const __grid_constant__ Table<TAB> T) {
+// the norm and the clip factor (at part[MAX_PARTS]) from the block sums, for lists that k_apply takes in many blocks
+__global__ void __launch_bounds__(1024) k_total(const __grid_constant__ Args A) {
+    __shared__ double sh[33];
+    after_previous();
+    double x = 0.0;
+    for (int i = threadIdx.x; i < A.nparts; i += 1024) x += A.part[i];
+    const double total = block_sum(x, sh);
+    if (threadIdx.x == 0) *reinterpret_cast<float*>(A.part + MAX_PARTS) = clip_factor(A, total, true);
+}
+
+// One block a chunk, the last chunk first.  SUM: every block adds the block sums up by itself.
+template <bool SUM, bool ADAM>
+__global__ void __launch_bounds__(THREADS, ADAM ? ADAM_CTAS : CLIP_CTAS) k_apply(const __grid_constant__ Args A, const __grid_constant__ Table<TAB> T) {
     __shared__ double sh[33];
     const Entry* tab = A.table ? A.table : T.e;
     after_previous();
-    double x = 0.0;
+    float c;
+    if (SUM) {
+        double x = 0.0;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < A.nparts; i += THREADS) x += A.part[i];
-    const double total = block_sum(x, sh);
-    const float c = clip_factor(A, total, blockIdx.x == 0 && threadIdx.x == 0);
-    apply_chunks(A, tab, c, blockIdx.x, gridDim.x);
+        for (int i = threadIdx.x; i < A.nparts; i += THREADS) x += A.part[i];
+        const double total = block_sum(x, sh);
+        c = clip_factor(A, total, blockIdx.x == 0 && threadIdx.x == 0);
+    } else {
+        c = *reinterpret_cast<const float*>(A.part + MAX_PARTS);
+    }
+    if (blockIdx.x < A.chunks) apply_chunk<ADAM>(A, tab, c, A.chunks - 1 - blockIdx.x);
 }
 
 // four neighbours of a tensor, the first `cnt` of them inside it; a wide access where the address and cnt allow it
@@ -433,7 +477,7 @@ static bool cluster_fits(int dev) {
 }
 
 static size_t ws_bytes(int n) {
-    return MAX_PARTS * sizeof(double) + (size_t)n * (sizeof(float2) + sizeof(Entry)) + 64;
+    return (MAX_PARTS + 1) * sizeof(double) + (size_t)n * (sizeof(float2) + sizeof(Entry)) + 64;
 }
 
 // two ranges of memory of one call may not share a byte: they are written by different blocks
@@ -467,7 +511,7 @@ static int run(const char* who, int n, void* const* g, const int* types, float* 
         const int es = types[i] == 0 ? 4 : 2;
         if (!g[i] || ((uintptr_t)g[i] & (es - 1))) return bad("null or misaligned gradient");
         ranges.emplace_back((uintptr_t)g[i], (uintptr_t)g[i] + (size_t)counts[i] * es);
-        Entry e = {g[i], nullptr, nullptr, nullptr, counts[i], 0, types[i], i};
+        Entry e = {g[i], nullptr, nullptr, nullptr, counts[i], 0, types[i], i, 0, 0};
         if (A.adam) {
             e.p = p[i]; e.m = m[i]; e.v = v[i];
             for (float* q : {e.p, e.m, e.v}) {
@@ -483,16 +527,26 @@ static int run(const char* who, int n, void* const* g, const int* types, float* 
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&nsm, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) { set_error((int)e, who, cudaGetErrorString(e)); return -1; }
-    // short chunks while there are too few long ones to give every resident block two
-    A.ch = total <= 2ll * nsm * CTAS_PER_SM * CH_BIG ? CH_SMALL : CH_BIG;
+    // chunks that give every resident block one, within bounds: a longer one keeps more loads in flight
+    const long long per = (total / ((long long)nsm * NORM_CTAS) + 1023) & ~1023ll;
+    A.ch = (int)std::min<long long>(CH_BIG, std::max<long long>(CH_SMALL, per));
     long long c0 = 0;
-    for (Entry& q : tab) { q.chunk0 = c0; c0 += (q.n + A.ch - 1) / A.ch; }
-    const bool small = A.ch == CH_SMALL && c0 <= CL * R && (A.adam ? cluster_fits<true>(dev) : cluster_fits<false>(dev));
+    for (Entry& q : tab) { q.chunk0 = c0; c0 += (q.n + CH_SMALL - 1) / CH_SMALL; }
+    const bool small = c0 <= CL * R && (A.adam ? cluster_fits<true>(dev) : cluster_fits<false>(dev));
+    if (!small) {
+        c0 = 0;
+        for (Entry& q : tab) {
+            const long long size = A.adam || q.type == 0 ? 4 : 2;
+            q.head = (int)std::min<long long>(q.n, (long long)(-(uintptr_t)(A.adam ? (void*)q.p : q.g) & 127) / size);
+            q.chunk0 = c0;
+            c0 += std::max(1ll, (q.n - q.head + A.ch - 1) / A.ch);
+        }
+    }
     A.chunks = c0;
     A.n = (int)tab.size();
     A.steps = steps;
     A.part = (double*)ws;
-    A.bias = (float2*)(A.part + MAX_PARTS);
+    A.bias = (float2*)(A.part + MAX_PARTS + 1);
     Table<TAB> T = {};
     A.table = nullptr;
     if (A.n <= TAB) {
@@ -503,7 +557,7 @@ static int run(const char* who, int n, void* const* g, const int* types, float* 
         for (int i = 0; i < A.n; i += TAB_BIG) {
             const int cnt = std::min(TAB_BIG, A.n - i);
             for (int k = 0; k < cnt; ++k) B.e[k] = tab[i + k];
-            e = go(1, k_table, 1, 256, st, B, cnt, dst + i);
+            e = go(1, k_table, (cnt + 15) / 16, 32, st, B, cnt, dst + i);
             if (e != cudaSuccess) break;
         }
         A.table = dst;
@@ -511,10 +565,17 @@ static int run(const char* who, int n, void* const* g, const int* types, float* 
     if (e == cudaSuccess && small) {
         e = A.adam ? go(CL, k_small<true>, CL, CL_THREADS, st, A, T) : go(CL, k_small<false>, CL, CL_THREADS, st, A, T);
     } else if (e == cudaSuccess) {
-        const int grid = (int)std::max(1ll, std::min<long long>(A.chunks, std::min(nsm * CTAS_PER_SM, MAX_PARTS)));
+        if (A.chunks >= (1ll << 31)) return bad("too many numbers");
+        const int grid = (int)std::max(1ll, std::min<long long>(A.chunks, std::min(nsm * NORM_CTAS, MAX_PARTS)));
         A.nparts = grid;
         e = go(1, k_norm, grid, THREADS, st, A, T);
-        if (e == cudaSuccess) e = go(1, k_apply, grid, THREADS, st, A, T);
+        if (A.chunks <= grid) {
+            if (e == cudaSuccess) e = A.adam ? go(1, k_apply<true, true>, grid, THREADS, st, A, T) : go(1, k_apply<true, false>, grid, THREADS, st, A, T);
+        } else {
+            if (e == cudaSuccess) e = go(1, k_total, 1, 1024, st, A);
+            const int all = (int)A.chunks;
+            if (e == cudaSuccess) e = A.adam ? go(1, k_apply<false, true>, all, THREADS, st, A, T) : go(1, k_apply<false, false>, all, THREADS, st, A, T);
+        }
     }
     if (e != cudaSuccess) { set_error((int)e, who, cudaGetErrorString(e)); return -1; }
     return 0;

@@ -317,41 +317,75 @@ def _rows(t):
 
 
 def _ff_args(x, w, b, act):
-    """Checked operands of a gated layer: rows [M, K] of x, w [2F, K] in x's type, b [2F] fp32 or None, and the codes of type
-    and activation."""
-    t, code = _FF_TYPE.get(x.dtype), _ACT.get(act)
-    dev = x.device
-    if dev.type != "cuda":
+    """Checked operands of a gated layer: rows [M, K] of x, w [2F, K] in x's type, b [2F] fp32 or None, F, and the codes of
+    type and activation."""
+    if not x.is_cuda:
         raise G1Error("a gated layer takes CUDA tensors (no CPU fallback)")
+    t, code, shape = _FF_TYPE.get(x.dtype), _ACT.get(act), w.shape
     if t is None:
         raise G1Error(f"a gated layer takes bf16 or fp16 rows, not {str(x.dtype)[6:]}")
     if w.dtype != x.dtype:
         raise G1Error("the weights must be of the rows' type")
     if code is None:
         raise G1Error(f"unknown activation {act!r} (one of {', '.join(_ACT)})")
-    if w.dim() != 2 or w.shape[0] % 2 or not w.numel() or x.dim() < 1 or x.shape[-1] != w.shape[1]:
+    if len(shape) != 2 or shape[0] % 2 or not shape[0] or not shape[1] or not x.dim() or x.shape[-1] != shape[1]:
         raise G1Error("a gated layer takes x [..., K] and w [2F, K]")
-    if w.device != dev or (b is not None and b.device != dev):
+    where = x.get_device()
+    if w.get_device() != where or (b is not None and b.get_device() != where):
         raise G1Error("a gated layer's tensors must be on one device")
     if b is not None:
-        if b.shape != w.shape[:1] or not b.is_floating_point():
+        if b.shape != shape[:1] or not b.is_floating_point():
             raise G1Error("the bias must be [2F]")
         if b.dtype != torch.float32:
             b = b.float()
         b = b.contiguous()
-    return _rows(x), _rows(w), b, t, code
+    return _rows(x), _rows(w), b, shape[0] // 2, t, code
 
 
-def _ff_ws(lib, x, w, F, backward):
-    """(M, K, address and row stride of x and of w), the bytes of the call's workspace and the workspace"""
+def _ff_operands(x, w):
+    """(M, K, address and row stride of x, of w)"""
     M, K = x.shape
-    px, ldx, pw, ldw = x.data_ptr(), x.stride(0) if M > 1 else K, w.data_ptr(), w.stride(0)
-    n = 0
-    if backward or (px | pw) & 15 or (ldx | ldw) & 7:   # else nothing has to be copied
-        n = lib.g1_gated_ff_workspace(M, K, F, px, ldx, pw, ldw, backward)
-        if n < 0 or M > 1 << 30:
-            raise G1Error("too many rows")
-    return M, K, px, ldx, pw, ldw, n, torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+    if M > 1 << 30:
+        raise G1Error("too many rows")
+    return M, K, x.data_ptr(), x.stride(0) if M > 1 else (K + 7) & ~7, w.data_ptr(), w.stride(0)
+
+
+def _bytes(x, n):
+    """A workspace of n bytes beside x (16-bit numbers)"""
+    return x.new_empty((n + 1) // 2) if n else None
+
+
+def _ff_forward(lib, dev, x, x2, w, b, F, t, code):
+    """h, and the operands as a backward call takes them: where their rows are not aligned, the copies that this call
+    leaves at the start of its workspace (the last of what is returned)."""
+    M, K, px, ldx, pw, ldw = _ff_operands(x2, w)
+    n, ws, copies = 0, None, None
+    if M > 4 and ((px | pw) & 15 or (ldx | ldw) & 7):
+        k8 = (K + 7) & ~7
+        nx = (M * k8 * 2 + 255) & ~255 if px & 15 or ldx & 7 else 0
+        nw = (F * k8 * 4 + 255) & ~255 if pw & 15 or ldw & 7 else 0
+        n = nx + nw
+        ws = _bytes(x, n)
+        at = ws.data_ptr()
+        copies = (M, K, at if nx else px, k8 if nx else ldx, at + nx if nw else pw, k8 if nw else ldw)
+    h = x.new_empty(x.shape[:-1] + (F,))
+    if lib.g1_gated_ff(M, K, F, t, code, px, ldx, pw, ldw, _addr(b), h.data_ptr(), _addr(ws), n, _stream_of(dev)):
+        _check()
+    return h, copies or (M, K, px, ldx, pw, ldw), ws
+
+
+def _ff_backward(lib, dev, dh, x, b, F, t, code, operands, need, dw_dtype):
+    M, K, px, ldx, pw, ldw = operands
+    n = lib.g1_gated_ff_workspace(M, K, F, px, ldx, pw, ldw, 1)
+    ws = _bytes(x, n)
+    dh = dh.contiguous()
+    dx = x.new_empty(x.shape) if need[0] else None
+    dw = x.new_empty((2 * F, K), dtype=dw_dtype) if need[1] else None
+    db = x.new_empty(2 * F, dtype=torch.float32) if need[2] else None
+    if lib.g1_gated_ff_backward(M, K, F, t, code, dh.data_ptr(), px, ldx, pw, ldw, _addr(b), _addr(dx), _addr(dw),
+                                _FF_TYPE.get(dw_dtype, 0), _addr(db), _addr(ws), n, _stream_of(dev)):
+        _check()
+    return dx, dw, db
 
 
 def _addr(t):
@@ -364,15 +398,10 @@ def gated_ff_device(x, w, b=None, act="silu"):
     Returns h [..., F] in x's type, on torch's current stream.  Rows may be strided; rows or weights that do
     not start on 16-byte boundaries (a row stride that is no multiple of 8) are copied first."""
     lib = load_library()
-    x2, w, b, t, code = _ff_args(x, w, b, act)
-    F = w.shape[0] // 2
+    x2, w, b, F, t, code = _ff_args(x, w, b, act)
     dev = x2.device
     with _on(dev):
-        M, K, px, ldx, pw, ldw, n, ws = _ff_ws(lib, x2, w, F, 0)
-        h = torch.empty(x.shape[:-1] + (F,), dtype=x.dtype, device=dev)
-        if lib.g1_gated_ff(M, K, F, t, code, px, ldx, pw, ldw, _addr(b), h.data_ptr(), _addr(ws), n, _stream_of(dev)):
-            _check()
-    return h
+        return _ff_forward(lib, dev, x, x2, w, b, F, t, code)[0]
 
 
 def gated_ff_backward_device(dh, x, w, b=None, act="silu", need=(True, True, True), dw_dtype=None):
@@ -380,8 +409,7 @@ def gated_ff_backward_device(dh, x, w, b=None, act="silu", need=(True, True, Tru
     or fp32), db [2F] fp32; None where `need` (dx, dw, db) says so.  Nothing of the forward pass but its inputs
     is needed.  dg and du are rounded to x's type before the products with W and x, but not in db."""
     lib = load_library()
-    x2, w, b, t, code = _ff_args(x, w, b, act)
-    F = w.shape[0] // 2
+    x2, w, b, F, t, code = _ff_args(x, w, b, act)
     dev = x2.device
     if dw_dtype is None:
         dw_dtype = x.dtype
@@ -390,19 +418,7 @@ def gated_ff_backward_device(dh, x, w, b=None, act="silu", need=(True, True, Tru
     if dh.device != dev or dh.dtype != x.dtype or dh.shape != x.shape[:-1] + (F,):
         raise G1Error("dh must be [..., F] on x's device and of its type")
     with _on(dev):
-        return _ff_backward(lib, dev, dh, x.shape, F, t, code, b, _ff_ws(lib, x2, w, F, 1), need, x.dtype, dw_dtype)
-
-
-def _ff_backward(lib, dev, dh, x_shape, F, t, code, b, operands, need, dtype, dw_dtype):
-    M, K, px, ldx, pw, ldw, n, ws = operands
-    dh = dh.contiguous()
-    dx = torch.empty(x_shape, dtype=dtype, device=dev) if need[0] else None
-    dw = torch.empty(2 * F, K, dtype=dw_dtype, device=dev) if need[1] else None
-    db = torch.empty(2 * F, dtype=torch.float32, device=dev) if need[2] else None
-    if lib.g1_gated_ff_backward(M, K, F, t, code, dh.data_ptr(), px, ldx, pw, ldw, _addr(b), _addr(dx), _addr(dw),
-                                _FF_TYPE.get(dw_dtype, 0), _addr(db), _addr(ws), n, _stream_of(dev)):
-        _check()
-    return dx, dw, db
+        return _ff_backward(lib, dev, dh, x, b, F, t, code, _ff_operands(x2, w), need, dw_dtype)
 
 
 def gated_ff_status():
@@ -415,35 +431,22 @@ class _GatedFF(torch.autograd.Function):
     def forward(ctx, x, w, b, act):
         lib = load_library()
         w16 = w if w.dtype == x.dtype else w.to(x.dtype)
-        x2, w2, b2, t, code = _ff_args(x, w16, b, act)
-        F, dev = w2.shape[0] // 2, x2.device
+        x2, w2, b2, F, t, code = _ff_args(x, w16, b, act)
+        dev = x2.device
         with _on(dev):
-            M, K, px, ldx, pw, ldw, n, ws = _ff_ws(lib, x2, w2, F, 0)
-            h = torch.empty(x.shape[:-1] + (F,), dtype=x.dtype, device=dev)
-            if lib.g1_gated_ff(M, K, F, t, code, px, ldx, pw, ldw, _addr(b2), h.data_ptr(), _addr(ws), n, _stream_of(dev)):
-                _check()
-        if n and M > 4:  # the backward pass takes the copies with aligned rows that this call left in ws
-            at, k8 = ws.data_ptr(), (K + 7) & ~7
-            if px & 15 or ldx & 7:
-                px, ldx = at, k8
-                at += (M * k8 * 2 + 255) & ~255
-            if pw & 15 or ldw & 7:
-                pw, ldw = at, k8
-        ctx.save_for_backward(x, w if w16 is w else w16, b)
-        ctx.call = (lib, dev, F, t, code, M, K, px, ldx, pw, ldw, w.dtype)
-        ctx.keep = (x2, w2, b2, ws)
+            h, operands, ws = _ff_forward(lib, dev, x, x2, w2, b2, F, t, code)
+        ctx.save_for_backward(x, w, b)
+        ctx.call = (lib, dev, b2, F, t, code, operands, w.dtype)
+        ctx.keep = (x2, w2, ws)  # what the operands' addresses are of
         return h
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
         x, w, b = ctx.saved_tensors  # notices a change made since
-        lib, dev, F, t, code, M, K, px, ldx, pw, ldw, w_dtype = ctx.call
-        need = ctx.needs_input_grad
+        lib, dev, b2, F, t, code, operands, w_dtype = ctx.call
         with _on(dev):
-            n = lib.g1_gated_ff_workspace(M, K, F, px, ldx, pw, ldw, 1)
-            ops = (M, K, px, ldx, pw, ldw, n, torch.empty(n, dtype=torch.uint8, device=dev))
-            dx, dw, db = _ff_backward(lib, dev, dh, x.shape, F, t, code, ctx.keep[2], ops, need, x.dtype, w_dtype)
+            dx, dw, db = _ff_backward(lib, dev, dh, x, b2, F, t, code, operands, ctx.needs_input_grad, w_dtype)
         return dx, dw, db if db is None or b.dtype == torch.float32 else db.to(b.dtype), None
 
 
@@ -539,20 +542,22 @@ def _dense(t):
     return t.permute(order).is_contiguous()
 
 
-def _cuda_list(tensors, what, types, dev=None):
-    """The device of a list of dense CUDA tensors of those types (dev where that is the one it must be)."""
-    for t in tensors:
-        if dev is None:
-            dev = t.device
-        if not t.is_cuda:
-            raise G1Error(f"{what} must be CUDA tensors")
-        if t.device != dev:
-            raise G1Error(f"{what} must be on one device")
-        if t.dtype not in types:
-            raise G1Error(f"{what} must be {' / '.join(str(x)[6:] for x in types)}, not {str(t.dtype)[6:]}")
-        if not t.is_contiguous() and not _dense(t):
-            raise G1Error(f"{what} must fill their memory without gaps (use .contiguous())")
-    return dev
+_T = torch.Tensor
+
+
+def _cuda_list(tensors, what, types):
+    """Checks a list of dense CUDA tensors of those types on one device; their device, None for an empty list."""
+    where = set(map(_T.get_device, tensors))
+    if -1 in where:
+        raise G1Error(f"{what} must be CUDA tensors")
+    if len(where) > 1:
+        raise G1Error(f"{what} must be on one device")
+    for t in {t.dtype for t in tensors}:
+        if t not in types:
+            raise G1Error(f"{what} must be {' / '.join(str(x)[6:] for x in types)}, not {str(t)[6:]}")
+    if not all(map(_T.is_contiguous, tensors)) and not all(map(_dense, tensors)):
+        raise G1Error(f"{what} must fill their memory without gaps (use .contiguous())")
+    return tensors[0].device if tensors else None
 
 
 def _array(ctype, values):
@@ -560,7 +565,7 @@ def _array(ctype, values):
 
 
 def _ptrs(tensors):
-    return _array(ctypes.c_void_p, [t.data_ptr() for t in tensors])
+    return _array(ctypes.c_void_p, list(map(_T.data_ptr, tensors)))
 
 
 def clip_grad_norm_device(grads, max_norm):
@@ -581,7 +586,7 @@ def clip_grad_norm_device(grads, max_norm):
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
     with _on(dev):
         rc = lib.g1_clip_grad_norm(n, _ptrs(grads), _array(ctypes.c_int, [_GRAD_TYPE[g.dtype] for g in grads]),
-                                   _array(ctypes.c_longlong, [g.numel() for g in grads]), max_norm, norm.data_ptr(),
+                                   _array(ctypes.c_longlong, list(map(_T.numel, grads))), max_norm, norm.data_ptr(),
                                    ws.data_ptr(), size, _stream_of(dev))
     if rc:
         _check()
@@ -625,6 +630,7 @@ class ClipAdam:
         self.steps = torch.full((len(self.params),), int(steps), dtype=torch.int64, device=self.device)
         self._counts = [p.numel() for p in self.params]
         self._strides = [p.stride() for p in self.params]
+        self._where = {self.device.index}
         self._state = self.exp_avg + self.exp_avg_sq + [self.steps]
 
     def zero_grad(self, set_to_none=True):
@@ -640,22 +646,34 @@ class ClipAdam:
         if len(grads) != n:
             raise G1Error("step takes one gradient (or None) a parameter")
         lib = _lib
-        ptrs, types, counts, moved = [None] * n, [0] * n, [0] * n, []
-        for i, g in enumerate(grads):
-            if g is None:
-                continue
-            p = params[i]
+        if (list(map(_T.stride, params)) != self._strides or list(map(_T.numel, params)) != self._counts
+                or set(map(_T.get_device, params)) != self._where or {p.dtype for p in params} != {torch.float32}):
+            raise G1Error("a parameter is no longer laid out as it was when the optimiser was made")
+        if any(g is None for g in grads):
+            have = [i for i, g in enumerate(grads) if g is not None]
+        else:
+            have = range(n)
+            if list(map(_T.stride, grads)) == self._strides and list(map(_T.numel, grads)) == self._counts:
+                have = ()  # nothing to look at one by one
+        for i in have:
+            g, p = grads[i], params[i]
             if g.shape != p.shape:
                 raise G1Error("gradients must have their parameters' shapes")
-            t = _GRAD_TYPE.get(g.dtype)
-            if t is None or g.device != dev:
-                raise G1Error("gradients must be fp32, bf16 or fp16 on their parameters' device")
-            if p.stride() != self._strides[i] or p.device != dev or p.dtype != torch.float32:
-                raise G1Error("a parameter is no longer laid out as it was when the optimiser was made")
             if g.stride() != self._strides[i]:
-                g = grads[i] = torch.empty_like(p, dtype=g.dtype, requires_grad=False).copy_(g.detach())
-            ptrs[i], types[i], counts[i] = g.data_ptr(), t, self._counts[i]
-            moved.append(p)
+                if not g.is_cuda:
+                    raise G1Error("gradients must be CUDA tensors")
+                grads[i] = torch.empty_like(p, dtype=g.dtype, requires_grad=False).copy_(g.detach())
+        there = grads if have == () else [g for g in grads if g is not None]
+        if not set(map(_T.get_device, there)) <= self._where or not {g.dtype for g in there} <= _GRAD_TYPE.keys():
+            raise G1Error("gradients must be fp32, bf16 or fp16 on their parameters' device")
+        if len(there) == n:
+            ptrs, types, counts = list(map(_T.data_ptr, grads)), [_GRAD_TYPE[g.dtype] for g in grads], self._counts
+            moved = params
+        else:
+            ptrs = [None if g is None else g.data_ptr() for g in grads]
+            types = [0 if g is None else _GRAD_TYPE[g.dtype] for g in grads]
+            counts = [0 if g is None else c for g, c in zip(grads, self._counts)]
+            moved = [p for p, g in zip(params, grads) if g is not None]
         norm = torch.empty((), dtype=torch.float32, device=dev)
         size = lib.g1_opt_workspace(n)
         ws = torch.empty(size, dtype=torch.uint8, device=dev)
