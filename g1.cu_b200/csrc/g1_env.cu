@@ -1057,11 +1057,11 @@ struct EnvState {
     __nv_bfloat16 *Xb, *Hb[2], *Wb;     // large-policy activations and weights
     float *Bf, *LS, *HD;
     int* derr;
-    size_t tc_N, tc_w, tc_wb;
+    size_t tc_N, tc_w, tc_wb, tc_b;
     int vnh, vhid[MAX_HIDDEN];          // separate value network (bf16 path), vnh = 0: shared trunk
     __nv_bfloat16* Wvb;
     float *Bvf, *HDv;
-    size_t tc_wvb, tc_hdv;
+    size_t tc_wvb, tc_bv, tc_hdv;
     uint8_t* tf_img;                    // fp32 policy on the tensor cores: chunk images + biases
     size_t tf_cap;
     int ffma_only;                      // 1: keep the fp32 policy on the FFMA path
@@ -1170,6 +1170,8 @@ static bool make_map(CUtensorMap* m, const void* base, int cols, int rows, int l
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+#include "g1_gated.cuh"
+
 template <int BN>
 static cudaError_t launch_gemm_tma(int M, int N, int K, const __nv_bfloat16* X, int ldx, const __nv_bfloat16* W,
                                    const float* bias, int act, float* of, int ldo, __nv_bfloat16* ob, int ldob, int* err,
@@ -1211,6 +1213,8 @@ static cudaError_t dense_tc(int M, int N, int K, const __nv_bfloat16* X, int ldx
 static void rollout_tc(EnvState* E, int H, const float* W, const float* mean, const float* var, float* O, float* A,
                        float* LP, float* V, float* R, float* D, float* Vlast) {
     const int N = E->N, nh = E->nh;
+    const bool gated = E->act >= 2;   // gated layers: W [2h][in], b [2h], the gate's rows first
+    const int per = gated ? 2 : 1;
     int maxw = 32;
     for (int l = 0; l < nh; ++l) maxw = E->hid[l] > maxw ? E->hid[l] : maxw;
     RepackPlan RP;
@@ -1220,13 +1224,13 @@ static void rollout_tc(EnvState* E, int H, const float* W, const float* mean, co
     int nin = OBS_DIM;
     for (int l = 0; l <= nh; ++l) {
         const bool head = l == nh;
-        const int no = head ? 32 : E->hid[l];
+        const int no = head ? 32 : per * E->hid[l];
         RP.srcW[l] = src; RP.nin[l] = nin; RP.ninp[l] = l == 0 ? XK : nin; RP.nout[l] = no;
         RP.srcB[l] = src + (long long)(head ? ACT_DIM : no) * nin;
         RP.dstW[l] = dw; RP.dstB[l] = db;
         dw += (long long)no * RP.ninp[l];
         db += no;
-        if (!head) { src += (long long)nin * no + no; nin = no; }
+        if (!head) { src += (long long)nin * no + no; nin = E->hid[l]; }
     }
     // separate value network: the policy part ends [.. Wmu, bmu, log_std], the value
     // network's layers and its 1-row output follow (g1env.pack_weights with value_hidden)
@@ -1242,22 +1246,22 @@ static void rollout_tc(EnvState* E, int H, const float* W, const float* mean, co
         VP.nl = E->vnh;
         for (int l = 0; l <= E->vnh; ++l) {
             const bool head = l == E->vnh;
-            const int no = head ? 32 : E->vhid[l];
+            const int no = head ? 32 : per * E->vhid[l];
             VP.srcW[l] = vs; VP.nin[l] = vin; VP.ninp[l] = l == 0 ? XK : vin; VP.nout[l] = no;
             VP.srcB[l] = vs + (long long)(head ? 1 : no) * vin;
             VP.dstW[l] = vdw; VP.dstB[l] = vdb;
             vdw += (long long)no * VP.ninp[l];
             vdb += no;
-            if (!head) { vs += (long long)vin * no + no; vin = no; }
+            if (!head) { vs += (long long)vin * no + no; vin = E->vhid[l]; }
             if (E->vhid[l] > maxw && !head) maxw = E->vhid[l];
         }
-        if (E->tc_wvb < (size_t)vdw || E->tc_hdv < (size_t)N) {
+        if (E->tc_wvb < (size_t)vdw || E->tc_bv < (size_t)vdb || E->tc_hdv < (size_t)N) {
             cudaFree(E->Wvb); cudaFree(E->Bvf); cudaFree(E->HDv);
-            E->Wvb = nullptr; E->Bvf = nullptr; E->HDv = nullptr; E->tc_wvb = 0; E->tc_hdv = 0;
+            E->Wvb = nullptr; E->Bvf = nullptr; E->HDv = nullptr; E->tc_wvb = 0; E->tc_bv = 0; E->tc_hdv = 0;
             CKR(cudaMalloc(&E->Wvb, (size_t)vdw * 2), );
             CKR(cudaMalloc(&E->Bvf, (size_t)vdb * 4), );
             CKR(cudaMalloc(&E->HDv, (size_t)N * 32 * 4), );
-            E->tc_wvb = vdw; E->tc_hdv = N;
+            E->tc_wvb = vdw; E->tc_bv = vdb; E->tc_hdv = N;
         }
     }
     // buffers (allocated on first use, kept by the env)
@@ -1270,12 +1274,12 @@ static void rollout_tc(EnvState* E, int H, const float* W, const float* mean, co
         CKR(cudaMalloc(&E->HD, (size_t)N * 32 * 4), );
         E->tc_N = N; E->tc_w = maxw;
     }
-    if (E->tc_wb < (size_t)dw) {
+    if (E->tc_wb < (size_t)dw || E->tc_b < (size_t)db) {
         cudaFree(E->Wb); cudaFree(E->Bf); cudaFree(E->LS);
         CKR(cudaMalloc(&E->Wb, (size_t)dw * 2), );
         CKR(cudaMalloc(&E->Bf, (size_t)db * 4), );
         CKR(cudaMalloc(&E->LS, 32 * 4), );
-        E->tc_wb = dw;
+        E->tc_wb = dw; E->tc_b = db;
     }
     if (!E->derr) { CKR(cudaMalloc(&E->derr, sizeof(int)), ); CKR(cudaMemset(E->derr, 0, sizeof(int)), ); }
     k_repack_bf16<<<240, 256, 0, E->stream>>>(W, E->Wb, E->Bf, E->LS, RP);
@@ -1291,6 +1295,10 @@ static void rollout_tc(EnvState* E, int H, const float* W, const float* mean, co
     P.o_vec = ((uintptr_t)O & 15) == 0;
     const dim3 oblk(32, 8);
     const int ogrid = (N + 7) / 8;
+    auto layer = [&](int width, int k, const __nv_bfloat16* in, const __nv_bfloat16* Wl, const float* bl, __nv_bfloat16* out) {
+        return gated ? g1ff::policy_layer(N, k, width, E->act, in, Wl, bl, out, E->sm_count, E->stream)
+                     : dense_tc(N, width, k, in, k, Wl, bl, E->act, nullptr, 0, out, width, E->derr, E->stream);
+    };
     auto policy = [&](int row, uint64_t tick) -> bool {
         k_obs_norm<<<ogrid, oblk, 0, E->stream>>>(P, row, E->Xb);
         if (cudaGetLastError() != cudaSuccess) return false;
@@ -1298,8 +1306,7 @@ static void rollout_tc(EnvState* E, int H, const float* W, const float* mean, co
         int k = XK;
         for (int l = 0; l < nh; ++l) {
             __nv_bfloat16* out = E->Hb[l & 1];
-            cudaError_t e = dense_tc(N, E->hid[l], k, in, k, E->Wb + RP.dstW[l], E->Bf + RP.dstB[l], E->act, nullptr, 0,
-                                     out, E->hid[l], E->derr, E->stream);
+            cudaError_t e = layer(E->hid[l], k, in, E->Wb + RP.dstW[l], E->Bf + RP.dstB[l], out);
             if (e != cudaSuccess) { set_error((int)e, "rollout_tc", cudaGetErrorString(e)); return false; }
             in = out;
             k = E->hid[l];
@@ -1312,8 +1319,7 @@ static void rollout_tc(EnvState* E, int H, const float* W, const float* mean, co
             k = XK;
             for (int l = 0; l < E->vnh; ++l) {
                 __nv_bfloat16* out = E->Hb[l & 1];
-                e = dense_tc(N, E->vhid[l], k, in, k, E->Wvb + VP.dstW[l], E->Bvf + VP.dstB[l], E->act, nullptr, 0, out,
-                             E->vhid[l], E->derr, E->stream);
+                e = layer(E->vhid[l], k, in, E->Wvb + VP.dstW[l], E->Bvf + VP.dstB[l], out);
                 if (e != cudaSuccess) { set_error((int)e, "rollout_tc", cudaGetErrorString(e)); return false; }
                 in = out;
                 k = E->vhid[l];
@@ -1342,6 +1348,12 @@ static int tc_error(EnvState* E) {
     int herr = 0;
     if (cudaMemcpy(&herr, E->derr, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return -1;
     if (herr) cudaMemset(E->derr, 0, sizeof(int));
+    if (E->act >= 2) {  // the gated layers' own flag, on the env's device
+        int dev = E->device;
+        if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(E->device) != cudaSuccess) return -1;
+        herr |= g1_gated_ff_status();
+        cudaSetDevice(dev);
+    }
     return herr;
 }
 
@@ -1483,7 +1495,7 @@ int g1_env_set_policy_ex(void* h, int nh, const int* hidden, int activation, int
         if (rc == 0) { E->prec = 0; E->ffma_only = precision == 2; }
         return rc;
     }
-    if (precision != 1 || nh < 1 || nh > MAX_HIDDEN || activation < 0 || activation > 1) {
+    if (precision != 1 || nh < 1 || nh > MAX_HIDDEN || activation < 0 || activation > 3) {
         set_error(-22, "g1_env_set_policy_ex", "invalid");
         return -22;
     }
@@ -1492,7 +1504,7 @@ int g1_env_set_policy_ex(void* h, int nh, const int* hidden, int activation, int
             set_error(-22, "g1_env_set_policy_ex", "bf16 widths must be multiples of 8 in [8, 1024]");
             return -22;
         }
-    E->nh = nh; E->act = activation; E->prec = 1;
+    E->nh = nh; E->act = activation; E->prec = 1;  // 2, 3: gated layers
     for (int i = 0; i < MAX_HIDDEN; ++i) E->hid[i] = i < nh ? hidden[i] : 0;
     return 0;
 }
@@ -1869,4 +1881,3 @@ void g1_occupancy_report(void) {
 // trainer batch preparation (GAE, observation renormalisation, RunNorm update)
 #include "g1_ppo_prep.cuh"
 #include "g1_opt.cuh"
-#include "g1_gated.cuh"

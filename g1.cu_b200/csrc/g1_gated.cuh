@@ -1145,6 +1145,14 @@ static cudaError_t backward(Call c, const Plan& L, const void* dh, void* dx, voi
     return e;
 }
 
+// a gated layer of the wide policies' rollout: bf16, rows and weights on 16-byte boundaries (K a multiple of 8)
+static cudaError_t policy_layer(int M, int K, int F, int act, const __nv_bfloat16* X, const __nv_bfloat16* W, const float* b,
+                                __nv_bfloat16* h, int nsm, cudaStream_t st) {
+    if (needs_pad(X, K) || needs_pad(W, K)) return cudaErrorInvalidValue;
+    const Call c = {M, K, F, 1, act, X, K, W, K, b, nullptr, st, nsm};
+    return forward<__nv_bfloat16>(c, plan(M, K, F, X, K, W, K, 0, nsm), h);
+}
+
 // tile indices are 32-bit
 static bool shape_ok(int M, int K, int F) {
     return M >= 0 && K >= 1 && F >= 1 && M <= (1 << 30) && K <= (1 << 20) && F <= (1 << 20) &&

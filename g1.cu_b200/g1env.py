@@ -161,10 +161,12 @@ class G1Env:
     def set_policy(self, hidden=(256, 256), activation="tanh", precision="fp32"):
         """precision "fp32": the in-kernel fp32-accurate policy (split-bf16 on the tensor cores when
         every hidden width is a multiple of 16 up to 256, else FFMA); "fp32-ffma": always FFMA;
-        "bf16": tensor-core policy for wide MLPs."""
+        "bf16": tensor-core policy for wide MLPs; with activation "swiglu" or "geglu"
+        of gated layers (AC of the same activation)."""
         hid = np.ascontiguousarray(hidden, np.int32)
         code = {"fp32": 0, "bf16": 1, "fp32-ffma": 2}[precision]
-        rc = _lib.g1_env_set_policy_ex(self.h, len(hidden), _dp(hid), 0 if activation == "tanh" else 1, code)
+        act = {"tanh": 0, "swiglu": 2, "geglu": 3}.get(activation, 1)
+        rc = _lib.g1_env_set_policy_ex(self.h, len(hidden), _dp(hid), act, code)
         if rc:
             _check()
 
@@ -753,14 +755,17 @@ class RunNorm:
 # ---------------- actor-critic (ppo.py:85-99) ----------------
 class AC(nn.Module):
     """The reference's actor-critic (shared trunk, value head on the last hidden layer).
-    value_hidden: a separate value network of those widths instead."""
+    value_hidden: a separate value network of those widths instead.
+    activation "swiglu" or "geglu": the hidden layers are GatedLinear, in bf16 on the tensor cores (CUDA only)."""
 
     def __init__(self, obs_dim, act_dim, hidden=(256, 256), activation="tanh", value_hidden=None):
         super().__init__()
         act = (lambda: nn.Tanh()) if activation == "tanh" else (lambda: nn.ELU())
+        gate = {"swiglu": "silu", "geglu": "gelu"}.get(activation)
+        layer = (lambda i, o: [GatedLinear(i, o, gate)]) if gate else (lambda i, o: [nn.Linear(i, o), act()])
         layers, d = [], obs_dim
         for h in hidden:
-            layers += [nn.Linear(d, h), act()]
+            layers += layer(d, h)
             d = h
         self.hidden = tuple(hidden)
         self.activation = activation
@@ -770,7 +775,7 @@ class AC(nn.Module):
         if self.value_hidden:
             vl, dv = [], obs_dim
             for h in self.value_hidden:
-                vl += [nn.Linear(dv, h), act()]
+                vl += layer(dv, h)
                 dv = h
             self.v_body = nn.Sequential(*vl)
             self.v = nn.Linear(dv, 1)
@@ -779,8 +784,9 @@ class AC(nn.Module):
         self.log_std = nn.Parameter(-0.5 * torch.ones(act_dim))
 
     def forward(self, x):
-        z = self.body(x)
-        v = self.v(self.v_body(x)) if self.value_hidden else self.v(z)
+        # gated layers answer in bf16; the heads are fp32
+        z = self.body(x).to(self.mu.weight.dtype)
+        v = self.v(self.v_body(x).to(self.v.weight.dtype)) if self.value_hidden else self.v(z)
         return self.mu(z), self.log_std.exp(), v.squeeze(-1)
 
 
@@ -788,8 +794,8 @@ def pack_weights(ac):
     """Flatten AC params in the order the kernel unpacks (ppo_fused.py:35-44): per hidden
     layer W,b; then Wmu,bmu, Wv,bv, log_std.  nn.Linear weight is [out,in] row-major.
     With a separate value network (g1_env_set_value_net): per policy hidden layer W,b; Wmu,
-    bmu, log_std; per value hidden layer W,b; Wv, bv."""
-    lin = lambda seq: [t for m in seq if isinstance(m, nn.Linear) for t in (m.weight.reshape(-1), m.bias)]
+    bmu, log_std; per value hidden layer W,b; Wv, bv.  A gated layer's W is [2h,in], its b [2h]."""
+    lin = lambda seq: [t for m in seq if isinstance(m, (nn.Linear, GatedLinear)) for t in (m.weight.reshape(-1), m.bias)]
     parts = lin(ac.body)
     if getattr(ac, "value_hidden", None):
         parts += [ac.mu.weight.reshape(-1), ac.mu.bias, ac.log_std] + lin(ac.v_body) + [ac.v.weight.reshape(-1), ac.v.bias]
@@ -803,7 +809,7 @@ def init_policy_normal(ac, seed=0):
     g = torch.Generator(device="cpu").manual_seed(seed)
     with torch.no_grad():
         for m in ac.modules():
-            if isinstance(m, nn.Linear):
+            if isinstance(m, (nn.Linear, GatedLinear)):
                 m.weight.copy_(torch.randn(m.weight.shape, generator=g) / np.sqrt(m.weight.shape[1]))
                 m.bias.zero_()
         ac.log_std.fill_(-0.5)

@@ -2,12 +2,18 @@
 training loop, ppo_fused.py:47-171, with world sharding across ranks).
 
     python g1.cu_b200/ppo_fused.py [iters] [n_worlds_per_gpu] [--smoke] [--tag=name] [--config4] [--no-eval] [--tf32]
+                                       [--gated] [--fused-opt]
     torchrun --nproc-per-node 8 g1.cu_b200/ppo_fused.py 1500 8192
     torchrun --nproc-per-node 8 g1.cu_b200/ppo_fused.py 3 65536 --config4 --no-eval
 
 --config4: policy 100-1024-1024-512-29 ELU on the bf16 tensor-core path plus a separate
 100-512-512-512-1 value network; each iteration prints its wall time split into rollout and
 update (and the rollout's substeps/s).
+
+--gated: the hidden layers are gated (SiLU) and run in bf16 on the tensor cores, in the rollout and in the update
+(g1_gated_ff, forward and backward); widths as without it.
+--fused-opt: the gradient norm, the clipping and the Adam step in one pass (ClipAdam, g1_clip_adam) in place of
+clip_grad_norm_ and torch.optim.Adam.
 
 The rollout runs in the CUDA library (g1_rollout); torch does only the PPO update, reading
 the trajectory buffers in place.  With WORLD_SIZE > 1 each rank owns its own worlds (global
@@ -26,7 +32,7 @@ import torch
 import torch.nn as nn
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from g1env import (AC, G1Env, RunNorm, adv_normalize_device, evaluate, gae_device, obs_prep_device,  # noqa: E402
+from g1env import (AC, ClipAdam, G1Env, RunNorm, adv_normalize_device, evaluate, gae_device, obs_prep_device,  # noqa: E402
                    pack_weights, runnorm_update_device)
 
 
@@ -111,7 +117,7 @@ def ppo_loss(ac, obs, act, old_logp, adv, ret, clip=0.2, vf_coef=0.5, ent_coef=0
 
 def ppo_update(ac, opt, b_o, b_a, b_lp, b_adv, b_ret, epochs=5, mb=4, clip=0.2):
     """Epochs x minibatches of ppo_loss over a shuffled batch, with the gradients averaged
-    over ranks before clipping (max norm 0.5) and the optimiser step."""
+    over ranks before clipping (max norm 0.5) and the optimiser step (a ClipAdam clips to its own max_norm in its step)."""
     n = b_o.shape[0]
     size = n // mb
     params = list(ac.parameters())
@@ -123,7 +129,8 @@ def ppo_update(ac, opt, b_o, b_a, b_lp, b_adv, b_ret, epochs=5, mb=4, clip=0.2):
             opt.zero_grad()
             loss.backward()
             allreduce_grads(params)
-            nn.utils.clip_grad_norm_(params, 0.5)
+            if not isinstance(opt, ClipAdam):
+                nn.utils.clip_grad_norm_(params, 0.5)
             opt.step()
             last = float(loss.item())
     return last
@@ -143,7 +150,7 @@ def main():
     iters = int(args[0]) if args else (3 if smoke else 1500)
     N = int(args[1]) if len(args) > 1 else (256 if smoke else 8192)
     H = 16 if smoke else 32
-    config4 = "--config4" in sys.argv
+    config4, gated = "--config4" in sys.argv, "--gated" in sys.argv
     do_eval = "--no-eval" not in sys.argv
     if "--tf32" in sys.argv:
         # opt-in: the update's matmuls on the tensor cores in TF32 (10-bit mantissa products,
@@ -157,15 +164,19 @@ def main():
     env = G1Env(N, substeps=10, pgs_iters=8, seed=1, device=local, world0=rank * N)
     O_dim, A_dim = env.obs_dim, env.act_dim
     torch.manual_seed(0)
+    hidden, value_hidden = ((1024, 1024, 512), (512, 512, 512)) if config4 else ((256, 256), None)
+    act = "swiglu" if gated else "elu" if config4 else "tanh"
+    if config4 or gated:
+        env.set_policy(hidden, act, precision="bf16")
     if config4:
-        env.set_policy((1024, 1024, 512), "elu", precision="bf16")
-        env.set_value_net((512, 512, 512))
-        ac = AC(O_dim, A_dim, (1024, 1024, 512), "elu", value_hidden=(512, 512, 512)).to(dev)
-    else:
-        ac = AC(O_dim, A_dim).to(dev)
+        env.set_value_net(value_hidden)
+    ac = AC(O_dim, A_dim, hidden, act, value_hidden=value_hidden).to(dev)
     broadcast_params(ac)
     norm = RunNorm(O_dim, dev)
-    opt = torch.optim.Adam(ac.parameters(), lr=3e-4)
+    if "--fused-opt" in sys.argv:
+        opt = ClipAdam(ac.parameters(), lr=3e-4, max_norm=0.5)
+    else:
+        opt = torch.optim.Adam(ac.parameters(), lr=3e-4)
     z = lambda *s: torch.zeros(*s, device=dev)
     O, A, LP, V, R, D, Vlast = z(H, N, O_dim), z(H, N, A_dim), z(H, N), z(H, N), z(H, N), z(H, N), z(N)
     env.reset()

@@ -101,7 +101,9 @@ int g1_env_set_policy(void* h, int nh, const int* hidden, int activation);
 
 /* extension: policy_precision 1 runs the MLP on the tensor cores (tcgen05, bf16 weights and
  * activations, fp32 accumulation) as separate launches per control step, for wide policies
- * (widths multiple of 8, up to 1024); 0 = the fp32 in-kernel policy of
+ * (widths multiple of 8, up to 1024), and with activation 2 (SiLU gate) or 3
+ * (GELU gate) as gated layers (g1_gated_ff): each hidden layer's packed weights are then W [2h,in]
+ * (gate rows, then up rows) and b [2h], in the value network too; 0 = the fp32 in-kernel policy of
  * g1_env_set_policy (computed with split-bf16 operands on the tensor cores -- fp32-class
  * accuracy -- when
  * every hidden width is a multiple of 16 in [16, 256], on FFMA otherwise); 2 = the fp32
