@@ -37,7 +37,7 @@ using g1gemm::s32;
 using g1gemm::tma_load_2d;
 
 constexpr int BM = 128, BK = 64;  // rows of A a CTA, chunk of the sum
-enum { FWD = 0, DZ = 1, DX = 2, DW = 3 };
+enum { FWD = 0, DZ = 1, DX = 2, DW = 3, DXS = 4 };  // DXS: DX with its sum cut, as DW's
 // CG: CTAs that work on a tile together (cta_group); BN: columns of B a tile
 template <int MODE, int BN, int CG>
 struct Cfg {
@@ -46,10 +46,9 @@ struct Cfg {
     static constexpr int PARTS = TN >= 64 ? 4 : TN / 16;           // epilogue warps a TMEM lane quarter
     static constexpr int EPI = 4 * PARTS, NTH = 64 + 32 * EPI;
     static constexpr int CW = TN / PARTS, SC = CW >= 32 ? 32 : 16; // columns a warp, and a step of it
-    static constexpr int LD = SC + 8;                              // 16-bit numbers a row of a warp's buffer (no bank conflicts)
     static constexpr int NB = BN / CG;                             // columns of B in this CTA's memory
-    static constexpr int STAGES = MODE == DZ ? 4 : MODE == DW ? 6 : 5;
-    static constexpr int BUFS = MODE == DZ ? 2 : MODE == DW ? 0 : 1;
+    static constexpr int STAGES = MODE == DZ ? 4 : MODE == FWD ? 5 : MODE == DX ? 6 : 7;
+    static constexpr int BUFS = MODE == DZ ? 2 : MODE == DW || MODE == DXS ? 0 : 1;
     static constexpr int STAGE_BYTES = (BM + NB) * BK * 2;
 };
 constexpr int DW_BLOCK = 64;  // chunks (of 64 rows) that the CTAs of DW walk together
@@ -65,7 +64,8 @@ struct Args {
     void* out;                   // h [M][F], z [M][2 Fp], dX [M][K], or the fp32 partial tiles
     long long ldo;
     float* db;                   // DZ: [gridDim][4][2F] column sums, or null
-    int tile0, ntp;              // DW: the pass's tiles
+    int tile0, ntp, blk;         // DW, DXS: the pass's tiles, chunks a block (see Tiles)
+    int direct, out32;           // DW: every CTA has the whole sum of its tile: dW itself is written, in fp32 or 16 bits
     int vec;                     // rows of the output and of dh are 16-byte aligned
 };
 
@@ -240,7 +240,7 @@ struct Smem {
     using C = Cfg<MODE, BN, CG>;
     uint8_t a[C::STAGES][BM * BK * 2];
     uint8_t b[C::STAGES][C::NB * BK * 2];
-    uint8_t buf[C::BUFS ? C::EPI : 1][C::BUFS ? C::BUFS : 1][C::BUFS ? 32 * C::LD * 2 : 16];
+    uint8_t buf[C::BUFS ? C::EPI : 1][C::BUFS ? C::BUFS : 1][C::BUFS ? 32 * C::SC * 2 : 16];
     float bias[C::PAIR ? C::EPI : 1][2][32];
     uint64_t full[C::STAGES], empty[C::STAGES], tfull[2], tempty[2];
     uint32_t tslot;
@@ -250,9 +250,14 @@ template <int MODE, int BN, int CG>
 constexpr int smem_bytes() { return (int)sizeof(Smem<MODE, BN, CG>) + 1024; }
 
 // A warp's 32 rows x SC columns go to and from global memory through its buffer, so that neighbouring lanes touch
-// neighbouring addresses: one row a lane would touch 32 lines with each access (measured on DZ, 524288 x 1024 x 512:
-// REPLACE_ME us that way).  vec: rows on 16-byte boundaries.
-template <class T, int SC, int LD>
+// neighbouring addresses (one row a lane would touch 32 lines with each access).  In the buffer the 16-byte groups of a
+// row are permuted so that a column group over 8 rows, and neighbouring groups, lie in different banks.
+template <int SC>
+__device__ __forceinline__ int at(int r, int group) {
+    return SC == 32 ? r * 64 + ((group ^ ((r >> 1) & 3)) << 4) : r * 32 + ((group ^ ((r >> 2) & 1)) << 4);
+}
+// to rows of m; vec: they start on 16-byte boundaries
+template <class T, int SC>
 __device__ __forceinline__ void rows_out(const uint8_t* buf, T* m, long long ld, int row0, int M, int col, int N, bool vec,
                                          int lane) {
     if (vec) {
@@ -263,7 +268,7 @@ __device__ __forceinline__ void rows_out(const uint8_t* buf, T* m, long long ld,
             const int r = lane / CH + i * (32 / CH);
             if (row0 + r < M && col + 8 * ch < N)
                 *reinterpret_cast<uint4*>(m + (size_t)(row0 + r) * ld + col + 8 * ch) =
-                    *reinterpret_cast<const uint4*>(buf + r * LD * 2 + ch * 16);
+                    *reinterpret_cast<const uint4*>(buf + at<SC>(r, ch));
         }
     } else {
         const int c = lane % SC;
@@ -271,10 +276,11 @@ __device__ __forceinline__ void rows_out(const uint8_t* buf, T* m, long long ld,
         for (int i = 0; i < SC; ++i) {
             const int r = lane / SC + i * (32 / SC);
             if (row0 + r < M && col + c < N)
-                m[(size_t)(row0 + r) * ld + col + c] = reinterpret_cast<const T*>(buf)[r * LD + c];
+                m[(size_t)(row0 + r) * ld + col + c] = *reinterpret_cast<const T*>(buf + at<SC>(r, c / 8) + c % 8 * 2);
         }
     }
 }
+
 // v[0..3] summed over the 8 lanes of equal l % 4: halves of the list change sides twice; lane l gets the sum of
 // v[2 (l / 16) + (l / 8) % 2]
 __device__ __forceinline__ float sums4(const float* v, int lane) {
@@ -300,7 +306,7 @@ __device__ __forceinline__ void fwd8(const uint32_t* rg, const uint32_t* ru, con
 }
 // z of 32 rows x 16 columns: dh in `buf` is replaced by dg, du goes to `buf2`; the column sums over the rows to s[k][]:
 // columns 8 k + 2 (l % 4), + 1 of dg, then of du
-template <class T, int ACT, int LD>
+template <class T, int ACT, int SC>
 __device__ __forceinline__ void dz16(const uint32_t (&rg)[2][8], const uint32_t (&ru)[2][8], const float (*sb)[32], int s0,
                                      uint8_t* buf, uint8_t* buf2, float (&sum)[2][4], int lane) {
 #pragma unroll
@@ -310,14 +316,14 @@ __device__ __forceinline__ void dz16(const uint32_t (&rg)[2][8], const uint32_t 
         f2 sg = 0, su = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int off = (((lane >> 2) + 8 * i) * LD + c) * 2;
-            uint32_t* at = reinterpret_cast<uint32_t*>(buf + off);
-            const f2 dh = mk(Half2<T>::unpack(*at));
+            const int off = at<SC>((lane >> 2) + 8 * i, s0 / 8 + k) + (lane & 3) * 4;
+            uint32_t* word = reinterpret_cast<uint32_t*>(buf + off);
+            const f2 dh = mk(Half2<T>::unpack(*word));
             f2 a, d;
             act2<ACT, true>(add(acc2(&rg[i / 2][4 * k + 2 * (i & 1)]), bg), a, d);
             const f2 dg = mul(mul(dh, add(acc2(&ru[i / 2][4 * k + 2 * (i & 1)]), bu)), d), du = mul(dh, a);
             const float2 x = un(dg), y = un(du);
-            *at = Half2<T>::pack(x.x, x.y);
+            *word = Half2<T>::pack(x.x, x.y);
             *reinterpret_cast<uint32_t*>(buf2 + off) = Half2<T>::pack(y.x, y.y);
             sg = add(sg, dg);
             su = add(su, du);
@@ -330,6 +336,27 @@ template <class T>
 __device__ __forceinline__ uint4 pack8(const float* v) {
     return make_uint4(Half2<T>::pack(v[0], v[1]), Half2<T>::pack(v[2], v[3]), Half2<T>::pack(v[4], v[5]),
                       Half2<T>::pack(v[6], v[7]));
+}
+
+// 16 neighbours of a row of dW, `n` of them inside it
+template <class T>
+__device__ __forceinline__ void store16(T* dst, const float* v, int n, bool vec) {
+    if (vec && n >= 16) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) reinterpret_cast<float4*>(dst)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        } else {
+            reinterpret_cast<uint4*>(dst)[0] = pack8<T>(v);
+            reinterpret_cast<uint4*>(dst)[1] = pack8<T>(v + 8);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (j < n) {
+                if constexpr (sizeof(T) == 4) dst[j] = v[j];
+                else dst[j] = Half2<T>::one(v[j]);
+            }
+    }
 }
 
 // ---- two CTAs on a tile
@@ -399,11 +426,11 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
 template <int MODE>
 struct Tiles {
     int tile, step, count, acc;      // FWD, DZ, DX
-    int t0, c0, c1, c2, blk;         // DW: chunks [c0, c1) of tile t0 and [0, c2) of tile t0 + 1 in each block
+    int t0, c0, c1, c2, blk;         // DW, DXS: chunks [c0, c1) of tile t0 and [0, c2) of tile t0 + 1 in each block
     // id-th of n CTAs (or groups of CTAs)
     __device__ __forceinline__ Tiles(const Args& P, int ntiles, int id, int n) {
-        if (MODE == DW) {
-            blk = min(DW_BLOCK, P.nk);
+        if (MODE == DW || MODE == DXS) {
+            blk = P.blk;
             const long long U = (long long)P.ntp * blk;
             const long long u0 = U * id / n, u1 = U * (id + 1) / n;
             t0 = (int)(u0 / blk);
@@ -423,7 +450,7 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
     using C = Cfg<MODE, BN, CG>;
     extern __shared__ uint8_t smem_raw[];
     auto& S = *reinterpret_cast<Smem<MODE, BN, CG>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    constexpr bool A_MN = MODE == DW, B_MN = MODE == DX || MODE == DW, PAIR = C::PAIR;
+    constexpr bool A_MN = MODE == DW, B_MN = MODE >= DX, PAIR = C::PAIR, CUT = MODE == DW || MODE == DXS;
     constexpr int TN = C::TN, STAGES = C::STAGES, NB = C::NB;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = CG == 1 ? 0 : (int)cta_rank();
@@ -487,7 +514,7 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                 } else {
                     load2d<CG>(bs, rank == 0 ? &P.b0 : &P.b1, c * BK, n0, bar);
                 }
-            } else if (MODE == DX) {
+            } else if (MODE == DX || MODE == DXS) {
                 // the sum runs over the gate half's columns, then the up half's
                 const bool up = c >= nk / 2;
                 const int k0 = (up ? c - nk / 2 : c) * BK;
@@ -506,7 +533,7 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
             if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             return true;
         };
-        if (MODE == DW) {
+        if (CUT) {
             for (int base = 0; base < nk && ok; base += W.blk) {
                 for (int c = W.c0; c < W.c1 && ok; ++c)
                     if (base + c < nk) ok = load(P.tile0 + W.t0, base + c);
@@ -537,7 +564,7 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
             if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             return true;
         };
-        if (MODE == DW) {
+        if (CUT) {
             for (int base = 0; base < nk && ok; base += W.blk) {
                 for (int c = W.c0; c < W.c1 && ok; ++c)
                     if (base + c < nk) ok = mma(tmem, base == 0 && c == W.c0);
@@ -557,9 +584,9 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
         }
     } else if (warp >= 2) {  // epilogue: warp w reads TMEM lanes 32 (w & 3) .., part (w - 2) / 4 of the columns
         const int q = warp & 3, part = (warp - 2) >> 2;
-        constexpr int CW = C::CW, SC = C::SC, LD = C::LD;
+        constexpr int CW = C::CW, SC = C::SC;
         const uint32_t tl = tmem + ((uint32_t)(32 * q) << 16);
-        if (MODE == DW) {
+        if (CUT) {
             // fp32 partial tiles, row-major; slot (group + tile) is this group's alone (the next share raises one of them)
             for (int a = 0; a < 2 && ok; ++a) {
                 const bool have = a == 0 ? W.c1 > W.c0 : W.c2 > 0;
@@ -571,11 +598,23 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                 asm volatile("tcgen05.fence::after_thread_sync;");
                 const size_t row = ((size_t)(blockIdx.x / CG + W.t0 + a) * CG + rank) * BM + 32 * q + lane;
                 float* dst = (float*)P.out + row * BN + part * CW;
+                const int tile = P.tile0 + W.t0 + a, mt = (tile / ntn) * CG + rank, up = mt >= half_tiles;
+                const int f = (up ? mt - half_tiles : mt) * BM + 32 * q + lane, k0 = (tile % ntn) * TN + part * CW;
 #pragma unroll 1
                 for (int cc = 0; cc < CW; cc += 16) {
                     uint32_t r[16];
                     tmem_ld16(tl + a * BN + part * CW + cc, r);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (MODE == DW && P.direct) {
+                        if (f >= P.F) continue;
+                        float v[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+                        const size_t at0 = (size_t)(up ? P.F + f : f) * P.N + k0 + cc;
+                        if (P.out32) store16((float*)P.out + at0, v, P.N - k0 - cc, P.vec);
+                        else store16((T*)P.out + at0, v, P.N - k0 - cc, P.vec);
+                        continue;
+                    }
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         reinterpret_cast<uint4*>(dst + cc)[j] = make_uint4(r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]);
@@ -640,6 +679,20 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                 asm volatile("tcgen05.fence::after_thread_sync;");
                 const int row0 = ((tile / ntn) * CG + rank) * BM + 32 * q;
                 const uint32_t t0 = tl + acc * BN + part * CW;
+                // hands the accumulator back once this warp has read its last columns of it
+                bool held = true;
+                auto release = [&]() {
+                    asm volatile("tcgen05.fence::before_thread_sync;");
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (CG == 1)
+                            asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s32(&S.tempty[acc])) : "memory");
+                        else
+                            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(acc ? tempty1 : tempty0)
+                                         : "memory");
+                    }
+                    held = false;
+                };
 #pragma unroll 1
                 for (int cc = 0; cc < CW; cc += SC) {
                     const int col = (tile % ntn) * TN + part * CW + cc;
@@ -650,11 +703,11 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                             if (P.vec) {
 #pragma unroll
                                 for (int i = 0; i < CH; ++i)
-                                    *reinterpret_cast<uint4*>(buf + (lane / CH + i * (32 / CH)) * LD * 2 + (lane % CH) * 16) = nx.v[i];
+                                    *reinterpret_cast<uint4*>(buf + at<SC>(lane / CH + i * (32 / CH), lane % CH)) = nx.v[i];
                             } else {
 #pragma unroll
                                 for (int i = 0; i < SC; ++i)
-                                    reinterpret_cast<uint16_t*>(buf)[(lane / SC + i * (32 / SC)) * LD + lane % SC] =
+                                    *reinterpret_cast<uint16_t*>(buf + at<SC>(lane / SC + i * (32 / SC), lane % SC / 8) + lane % 8 * 2) =
                                         (uint16_t)(nx.w[i / 2] >> (16 * (i & 1)));
                             }
                         }
@@ -663,7 +716,6 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                     if (cc + SC < CW) ask(tile, cc + SC);
                     else ask(tile + W.step, 0);
                     if (!some) continue;
-                    uint8_t* mine = buf + lane * LD * 2;
 #pragma unroll 1
                     for (int s = 0; s < SC; s += 16) {
                         if (MODE == DZ) {
@@ -673,11 +725,12 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                             tmem_ld16x16(t0 + TN + cc + s, ru[0]);
                             tmem_ld16x16(t0 + (16u << 16) + TN + cc + s, ru[1]);
                             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                            if (cc + s + 16 == CW) release();
                             float sum[2][4];
-                            if (P.act == 0) dz16<T, 0, LD>(rg, ru, sb, s, buf, buf2, sum, lane);
-                            else if (P.act == 1) dz16<T, 1, LD>(rg, ru, sb, s, buf, buf2, sum, lane);
-                            else if (P.act == 2) dz16<T, 2, LD>(rg, ru, sb, s, buf, buf2, sum, lane);
-                            else dz16<T, 3, LD>(rg, ru, sb, s, buf, buf2, sum, lane);
+                            if (P.act == 0) dz16<T, 0, SC>(rg, ru, sb, s, buf, buf2, sum, lane);
+                            else if (P.act == 1) dz16<T, 1, SC>(rg, ru, sb, s, buf, buf2, sum, lane);
+                            else if (P.act == 2) dz16<T, 2, SC>(rg, ru, sb, s, buf, buf2, sum, lane);
+                            else dz16<T, 3, SC>(rg, ru, sb, s, buf, buf2, sum, lane);
                             if (P.db) {  // rows behind the last one have dh = 0
 #pragma unroll
                                 for (int k = 0; k < 2; ++k) {
@@ -694,6 +747,7 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                         uint32_t ru[16];
                         if (MODE == FWD) tmem_ld16(t0 + TN + cc + s, ru);
                         asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                        if (cc + s + 16 == CW) release();
 #pragma unroll
                         for (int e = 0; e < 16; e += 8) {
                             float h[8];
@@ -711,24 +765,16 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
 #pragma unroll
                                 for (int j = 0; j < 8; ++j) h[j] = __uint_as_float(r[e + j]);
                             }
-                            *reinterpret_cast<uint4*>(mine + (s + e) * 2) = pack8<T>(h);
+                            *reinterpret_cast<uint4*>(buf + at<SC>(lane, (s + e) / 8)) = pack8<T>(h);
                         }
                     }
                     __syncwarp();
                     // z's rows are padded to whole 16-byte groups
-                    rows_out<T, SC, LD>(buf, (T*)P.out, P.ldo, row0, P.M, col, P.N, MODE == DZ || P.vec, lane);
-                    if (MODE == DZ) rows_out<T, SC, LD>(buf2, (T*)P.out + P.ldo / 2, P.ldo, row0, P.M, col, P.N, true, lane);
+                    rows_out<T, SC>(buf, (T*)P.out, P.ldo, row0, P.M, col, P.N, MODE == DZ || P.vec, lane);
+                    if (MODE == DZ) rows_out<T, SC>(buf2, (T*)P.out + P.ldo / 2, P.ldo, row0, P.M, col, P.N, true, lane);
                     __syncwarp();
                 }
-                asm volatile("tcgen05.fence::before_thread_sync;");
-                __syncwarp();
-                if (lane == 0) {
-                    if (CG == 1)
-                        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s32(&S.tempty[acc])) : "memory");
-                    else
-                        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(acc ? tempty1 : tempty0)
-                                     : "memory");
-                }
+                if (held) release();  // columns behind the last one
                 if (++acc == 2) { acc = 0; accph ^= 1u; }
             }
         }
@@ -768,26 +814,23 @@ __device__ __forceinline__ void db_sum(const float* part, float* db, int rows, i
 }
 
 // dW from the partial tiles: tile t is the sum of the slots b + t of the groups of CTAs whose shares of a block's units meet
-// it, in the order of b.  One thread, 4 columns; grid: (rows of a tile) x tiles.  Further blocks (blockIdx.y = ntp, or 0
-// where ntp is 0) sum db.
+// it, in the order of b.  One thread, 4 columns; grid: (rows of a tile) x tiles.  Further blocks (blockIdx.y >= ntp)
+// sum db.
 template <class T, int BN, int CG>
 __global__ void __launch_bounds__(256) k_dw_sum(const float* part, T* dw, int F, int K, int tile0, int ntp, int blk, int groups,
                                                 int ntn, const float* db_part, float* db, int db_rows) {
     constexpr int C4 = BN / 4, R = BM * CG;
     const int t = blockIdx.y;
-    if (t == ntp) {
+    if (t >= ntp) {
         after_previous();
-        for (int b = blockIdx.x; b * 8 < 2 * F; b += gridDim.x) {
-            db_sum(db_part, db, db_rows, 2 * F, b);
-            __syncthreads();
-        }
+        db_sum(db_part, db, db_rows, 2 * F, (t - ntp) * gridDim.x + blockIdx.x);
         return;
     }
     const int idx = blockIdx.x * 256 + threadIdx.x, r = idx / C4, c = (idx % C4) * 4;
     const int tile = tile0 + t, half_tiles = (F + BM - 1) / BM;
     const int mt = (tile / ntn) * CG + r / BM, up = mt >= half_tiles;
     const int f = (up ? mt - half_tiles : mt) * BM + r % BM, k = (tile % ntn) * BN + c;
-    const int U = ntp * blk, lo = t * blk, hi = lo + blk;  // U x groups stays below 2^31: 148 tiles, 64 chunks, 148 groups
+    const int U = ntp * blk, lo = t * blk, hi = lo + blk;  // U x groups stays below 2^31 (checked where it is launched)
     int b0 = lo * groups / U, b1 = hi * groups / U;
     while (b0 > 0 && U * b0 / groups > lo) --b0;           // the group whose share holds lo ..
     while (U * (b0 + 1) / groups <= lo) ++b0;
@@ -958,13 +1001,14 @@ static int pad8(int n) { return (n + 7) & ~7; }
 constexpr int ROWS_MAX = 4;  // rows up to which the forward pass goes by k_ff_rows
 
 // Columns of B a tile, for `cols` output columns that B has `per` of for each: 256 on pairs of CTAs (cg 2) where that
-// gives every pair a tile, else 128 or 64 on single ones, the narrower the fewer tiles there are.
+// gives two of three pairs a tile, else 128 or 64 on single ones, the narrower the fewer tiles there are.  Measured, forward:
+// 2048 x 1024 x 1024 (64 pair tiles) 12.0 us on pairs, 15.9 on single CTAs; 1024 x 1024 x 1024 (32) 11.0 and 9.8.
 struct Shape {
     int bn, cg;
 };
 static Shape tile_shape(int M, int cols, int per, int nsm) {
     auto tiles = [&](int rows, int bn) { return (long long)((M + rows - 1) / rows) * ((cols * per + bn - 1) / bn); };
-    if (cols * per > 128 && tiles(2 * BM, 256) * 2 >= nsm) return {256, 2};
+    if (cols * per > 128 && tiles(2 * BM, 256) * 3 >= nsm) return {256, 2};
     if (cols * per > 64 && tiles(BM, 128) * 2 > nsm) return {128, 1};
     return {64, 1};
 }
@@ -974,7 +1018,16 @@ struct Plan {
     bool padx, padw;
     Shape dw;
     int tiles, passes, ntp, groups, blk;
+    bool direct;
+    Shape dx;
+    int dx_tiles, dx_groups;  // dx_groups: 0 where the sum of DX is not cut
 };
+// Whether a sum of nk chunks for each of `tiles` tiles is cut over `all` groups of CTAs: it saves the idle groups' share of the
+// time (a chunk takes some 0.25 us) and costs the partial tiles' way through memory and a launch, some 10 us.
+// Measured, backward in a graph: 512 x 104 x 2048 with cut sums 33 us, with whole ones 86 to 114 (dX: 4 tiles, 64 chunks);
+// 4096 x 2048 x 2048 with whole ones 182, with cut ones 253 (dW: 2 passes of 64 tiles).
+static bool worth_cutting(int nk, long long tiles, int all) { return tiles < all && nk * (all - tiles) >= 40ll * all; }
+
 // DW: passes of at most one tile a group of CTAs (then its share meets two tiles at most)
 static Plan plan(int M, int K, int F, const void* X, long long ldx, const void* W, long long ldw, int backward, int nsm) {
     Plan L = {};
@@ -988,17 +1041,33 @@ static Plan plan(int M, int K, int F, const void* X, long long ldx, const void* 
     if (backward) {
         L.z = take((long long)M * 2 * pad8(F) * 2);
         L.db = take((long long)nsm * 4 * 2 * F * 4);
-        L.dw = K <= 64 ? Shape{64, 1} : K <= 128 ? Shape{128, 1} : Shape{256, 2};
+        const int nk = (M + BK - 1) / BK;
+        // a short sum: small tiles on all SMs, as it is the writing of dW that takes the time
+        L.dw = K <= 64 ? Shape{64, 1} : K <= 128 || nk <= 8 ? Shape{128, 1} : Shape{256, 2};
         const int all = nsm / L.dw.cg;
         L.tiles = 2 * ((F + BM - 1) / BM) / L.dw.cg * ((K + L.dw.bn - 1) / L.dw.bn);
         L.passes = (L.tiles + all - 1) / all;
         L.ntp = (L.tiles + L.passes - 1) / L.passes;
-        const int nk = (M + BK - 1) / BK;
         L.blk = nk < DW_BLOCK ? nk : DW_BLOCK;
+        // (rows of dW that start anywhere are written number by number, a row a lane, where no sum follows: not for long)
+        L.direct = !worth_cutting(nk, L.ntp, all) && (K % 8 == 0 || nk <= 4);
+        // four chunks a share at least
         const long long units = (long long)L.ntp * L.blk;
-        // four chunks a share at least: below that its partial tile costs more than its products
-        L.groups = (int)std::min<long long>(all, std::max<long long>(L.ntp, units / 4));
-        L.part = take((long long)(L.groups + L.ntp) * L.dw.cg * BM * L.dw.bn * 4);
+        L.groups = L.direct ? L.ntp : (int)std::min<long long>(all, std::max<long long>(L.ntp, units / 4));
+        long long part = L.direct ? 0 : (long long)(L.groups + L.ntp) * L.dw.cg * BM * L.dw.bn * 4;
+        L.dx = tile_shape(M, K, 1, nsm);
+        const int nkx = 2 * ((F + BK - 1) / BK);
+        if (L.dx.cg == 1) {
+            const Shape cut = K <= 64 ? Shape{64, 1} : Shape{128, 1};
+            const long long tiles = (long long)((M + BM - 1) / BM) * ((K + cut.bn - 1) / cut.bn);
+            if (worth_cutting(nkx, tiles, nsm)) {
+                L.dx = cut;
+                L.dx_tiles = (int)tiles;
+                L.dx_groups = (int)std::min<long long>(nsm, tiles * nkx / 4);
+                part = std::max(part, (long long)(L.dx_groups + L.dx_tiles) * BM * cut.bn * 4);
+            }
+        }
+        L.part = take(part);
     }
     L.total = o;
     return L;
@@ -1070,26 +1139,39 @@ static cudaError_t forward(Call c, const Plan& L, void* h) {
     return pair_tiles<T, FWD>(c, P, &ctas);
 }
 
+// sums partial tiles (of dX as of dW); the last blocks sum db where it is given
+template <class T, class O, int BN, int CG>
+static cudaError_t sum_tiles(const Call& c, const float* part, O* out, int rows, int tile0, int ntp, int blk, int groups,
+                             const float* db_part, float* db, int db_rows) {
+    if ((long long)ntp * blk * (groups + 1) >= (1ll << 31)) return cudaErrorInvalidValue;
+    const int x = CG * BM * BN / 4 / 256;
+    const dim3 grid(x, ntp + (db ? ((2 * c.F + 7) / 8 + x - 1) / x : 0));
+    if (grid.y > 65535) return cudaErrorInvalidValue;
+    return go(1, k_dw_sum<O, BN, CG>, grid, 256, 0, c.st, part, out, rows, c.K, tile0, ntp, blk, groups, (c.K + BN - 1) / BN, db_part,
+              db, db_rows);
+}
+
 template <class T, int BN, int CG>
 static cudaError_t dw_passes(const Call& c, const Plan& L, Args P, void* dw, int dw_type, const float* db_part, float* db, int db_rows) {
-    const int ntn = (c.K + BN - 1) / BN;
+    P.blk = L.blk;
+    P.direct = L.direct;
+    P.out32 = dw_type == 0;
+    P.out = L.direct ? dw : c.ws + L.part;
+    P.vec = c.K % 8 == 0 && ((uintptr_t)dw & 15) == 0;
+    const float* part = (const float*)P.out;
     for (int t0 = 0; t0 < L.tiles; t0 += L.ntp) {
         P.tile0 = t0;
         P.ntp = std::min(L.ntp, L.tiles - t0);
-        const int groups = (int)std::min<long long>((long long)P.ntp * L.blk, L.groups);
-        static_assert(148ll * DW_BLOCK * 148 < (1ll << 31), "k_dw_sum's products");
+        const int groups = L.direct ? P.ntp : (int)std::min<long long>((long long)P.ntp * L.blk, L.groups);
         cudaError_t e = launch<T, DW, BN, CG>(P, groups, c.st);
         if (e != cudaSuccess) return e;
-        const dim3 grid(CG * BM * BN / 4 / 256, P.ntp + (db ? 1 : 0));
-        const float* part = (const float*)P.out;
-        e = dw_type == 0 ? go(1, k_dw_sum<float, BN, CG>, grid, 256, 0, c.st, part, (float*)dw, c.F, c.K, t0, P.ntp, L.blk, groups,
-                              ntn, db_part, db, db_rows)
-                         : go(1, k_dw_sum<T, BN, CG>, grid, 256, 0, c.st, part, (T*)dw, c.F, c.K, t0, P.ntp, L.blk, groups, ntn,
-                              db_part, db, db_rows);
-        db = nullptr;  // with the first pass
+        if (L.direct) continue;
+        e = dw_type == 0 ? sum_tiles<T, float, BN, CG>(c, part, (float*)dw, c.F, t0, P.ntp, L.blk, groups, db_part, db, db_rows)
+                         : sum_tiles<T, T, BN, CG>(c, part, (T*)dw, c.F, t0, P.ntp, L.blk, groups, db_part, db, db_rows);
         if (e != cudaSuccess) return e;
+        db = nullptr;  // with the first pass
     }
-    return cudaSuccess;
+    return db ? sum_tiles<T, T, 64, 1>(c, nullptr, (T*)nullptr, c.F, 0, 0, 1, 1, db_part, db, db_rows) : cudaSuccess;
 }
 
 template <class T>
@@ -1119,12 +1201,24 @@ static cudaError_t backward(Call c, const Plan& L, const void* dh, void* dx, voi
         P.nk = 2 * ((c.F + BK - 1) / BK);
         P.out = dx; P.ldo = c.K;
         P.vec = c.K % 8 == 0 && ((uintptr_t)dx & 15) == 0;
-        const Shape sh = tile_shape(c.M, c.K, 1, c.nsm);
-        const int rows = BM * sh.cg;
-        const int groups = (int)std::min<long long>((long long)((c.M + rows - 1) / rows) * ((c.K + sh.bn - 1) / sh.bn), c.nsm / sh.cg);
-        e = sh.bn == 64    ? launch<T, DX, 64, 1>(P, groups, c.st)
-            : sh.bn == 128 ? launch<T, DX, 128, 1>(P, groups, c.st)
-                           : launch<T, DX, 256, 2>(P, groups, c.st);
+        const Shape sh = L.dx;
+        if (L.dx_groups) {
+            P.blk = P.nk;
+            P.ntp = L.dx_tiles;
+            P.out = c.ws + L.part;
+            e = sh.bn == 64 ? launch<T, DXS, 64, 1>(P, L.dx_groups, c.st) : launch<T, DXS, 128, 1>(P, L.dx_groups, c.st);
+            if (e != cudaSuccess) return e;
+            const float* part = (const float*)P.out;
+            // as dW's gate half: M rows
+            e = sh.bn == 64 ? sum_tiles<T, T, 64, 1>(c, part, (T*)dx, c.M, 0, P.ntp, P.blk, L.dx_groups, nullptr, nullptr, 0)
+                            : sum_tiles<T, T, 128, 1>(c, part, (T*)dx, c.M, 0, P.ntp, P.blk, L.dx_groups, nullptr, nullptr, 0);
+        } else {
+            const int rows = BM * sh.cg;
+            const int groups = (int)std::min<long long>((long long)((c.M + rows - 1) / rows) * ((c.K + sh.bn - 1) / sh.bn), c.nsm / sh.cg);
+            e = sh.bn == 64    ? launch<T, DX, 64, 1>(P, groups, c.st)
+                : sh.bn == 128 ? launch<T, DX, 128, 1>(P, groups, c.st)
+                               : launch<T, DX, 256, 2>(P, groups, c.st);
+        }
         if (e != cudaSuccess) return e;
     }
     if (dw) {
@@ -1134,14 +1228,11 @@ static cudaError_t backward(Call c, const Plan& L, const void* dh, void* dx, voi
             return cudaErrorInvalidValue;
         P.M = c.M; P.N = c.K; P.F = c.F;
         P.nk = (c.M + BK - 1) / BK;
-        P.out = c.ws + L.part;
         return L.dw.bn == 64    ? dw_passes<T, 64, 1>(c, L, P, dw, dw_type, db_part, db, ctas * 4)
                : L.dw.bn == 128 ? dw_passes<T, 128, 1>(c, L, P, dw, dw_type, db_part, db, ctas * 4)
                                 : dw_passes<T, 256, 2>(c, L, P, dw, dw_type, db_part, db, ctas * 4);
     }
-    if (db)
-        e = go(1, k_dw_sum<T, 64, 1>, dim3((2 * c.F + 7) / 8, 1), 256, 0, c.st, (const float*)nullptr, (T*)nullptr, c.F, c.K, 0, 0, 0, 1,
-               1, db_part, db, ctas * 4);
+    if (db) e = sum_tiles<T, T, 64, 1>(c, nullptr, (T*)nullptr, c.F, 0, 0, 1, 1, db_part, db, ctas * 4);
     return e;
 }
 
