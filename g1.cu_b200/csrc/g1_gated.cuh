@@ -9,7 +9,9 @@
 // operands of the tensor cores there): half a step of each term, which averages over the sum and stays below
 // the result's own rounding; db is summed from the unrounded values.
 //
-// One kernel, k_ff, in four modes, all C = A B over 128 x BN tiles with fp32 accumulators in tensor memory:
+// One kernel, k_ff, in several modes, all C = A B with fp32 accumulators in tensor memory, on 256 x 256 tiles by pairs of
+// CTAs (cta_group::2: each CTA loads its 128 rows of A and half of B), or 128 x 128 / 64 by single ones where there
+// are too few of those (tile_shape):
 //
 //   FWD  A = X, B = 128 rows of Wg and the same 128 rows of Wu, one MMA of N = 256; the epilogue holds g and u of
 //        128 outputs side by side and writes h.  Neither g nor u leaves the SM.
@@ -19,12 +21,25 @@
 //        or so, and hold 8 bytes an output between forward and backward.
 //   DX   A = z, B = W read along its rows (MN-major): no transposed copy.
 //   DW   A = z^T, B = X^T, both MN-major straight from their row-major tiles, summed over M.  The 2F x K tiles are
-//        few and M is long: see the work split at k_ff's iterator.
+//        few and M is long: the work split stands at Tiles.  DXS: DX split the same way, for few rows and many outputs.
+//   A few rows (up to ROWS_MAX) go forward by k_ff_rows, without tensor cores.
 //
-// Operands come by TMA (128-byte swizzle, zero fill past the edges, no multicast) in chunks of 64 along the sum,
-// four stages; one thread issues the loads, one the MMAs, sixteen warps run the epilogue of a tile while the
+// Operands come by TMA (128-byte swizzle, zero fill past the edges, no multicast) in chunks of 64 along the sum, four to seven
+// stages; one thread issues the loads, one the MMAs, up to sixteen warps run the epilogue of a tile while the
 // next one accumulates in the other half of tensor memory.  Every wait is bounded; one that runs out sets g_err
 // (g1_gated_ff_status), and the kernel ends with garbage in its outputs.
+//
+// What bounds it: the products.  A chunk's 32 KB a CTA are written to and read from shared memory in the 512 cycles of its
+// MMAs, close to the 128 bytes a cycle that it has (tensor pipe 74 % active in DX, 56 % in DZ, whose epilogue moves
+// dh, dg and du through shared memory as well); under the power cap of a long step the clock gives way first.
+// Measured on one B200 (graph replays; percent of the measured 1659 TFLOP/s):
+//   forward 32768 x 1024 x 1024                       101 us   1363 TFLOP/s   82 %
+//   forward and backward 524288 x 1024 x 512         3.69 to 4.0 ms, by box: FWD 0.80, DZ 0.98, DX 0.83, DW 0.83 alone;
+//                                                    860 TFLOP/s of the 12MKF that cannot be avoided, 1146 of the 16MKF run
+//   forward 1 x 1024 x 1024                           2.1 us   2.0 TB/s from L2: latency
+// Steps: 128-row tiles by single CTAs 117 us and 4.57 ms; pairs of CTAs 109 us and 4.29 ms; coalesced epilogue with
+// two-number arithmetic 101 us and 3.9 ms; accumulators handed back before the stores, no bank conflicts 3.7 ms.  Fetching
+// the next tile's A to L2 a tile ahead made it 115 us and 4.6 ms and was taken out.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -34,7 +49,6 @@
 namespace g1ff {
 
 using g1gemm::s32;
-using g1gemm::tma_load_2d;
 
 constexpr int BM = 128, BK = 64;  // rows of A a CTA, chunk of the sum
 enum { FWD = 0, DZ = 1, DX = 2, DW = 3, DXS = 4 };  // DXS: DX with its sum cut, as DW's
@@ -425,10 +439,10 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
 // once; cutting each tile's whole M into runs instead would have the tiles read the same rows at different times.
 template <int MODE>
 struct Tiles {
-    int tile, step, count, acc;      // FWD, DZ, DX
+    int tile, step;                  // FWD, DZ, DX
     int t0, c0, c1, c2, blk;         // DW, DXS: chunks [c0, c1) of tile t0 and [0, c2) of tile t0 + 1 in each block
     // id-th of n CTAs (or groups of CTAs)
-    __device__ __forceinline__ Tiles(const Args& P, int ntiles, int id, int n) {
+    __device__ __forceinline__ Tiles(const Args& P, int id, int n) {
         if (MODE == DW || MODE == DXS) {
             blk = P.blk;
             const long long U = (long long)P.ntp * blk;
@@ -440,7 +454,6 @@ struct Tiles {
         } else {
             tile = id;
             step = n;
-            count = ntiles;
         }
     }
 };
@@ -492,7 +505,7 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
     const uint32_t tmem = S.tslot;
     bool ok = true;
     after_previous();
-    const Tiles<MODE> W(P, ntiles, blockIdx.x / CG, gridDim.x / CG);
+    const Tiles<MODE> W(P, blockIdx.x / CG, gridDim.x / CG);
 
     if (warp == 0 && lane == 0) {  // loads: this CTA's rows of A and its share of B
         int stage = 0;
@@ -879,7 +892,8 @@ __global__ void __launch_bounds__(256) k_pad(PadJob a, PadJob b, int ldd, int n)
 
 // The forward pass of a few rows (a world or some asking for their next action): the weights' bytes are the work, and
 // 128-row tiles would leave it to F / 32 CTAs at most.  One warp an output: it reads row f of Wg and of Wu once, 16 bytes
-// a lane (VEC; single numbers where rows start anywhere), the rows of X come from L1.  R rows at a time.
+// a lane (VEC; single numbers where rows start anywhere), the rows of X come from L1.  R rows at a time.  Measured in a
+// graph, this and 128-row tiles: 1 x 1024 x 1024 2.1 us and 8.1, 4 rows 5.7 and 8.1 (8 rows took 9.9)
 template <class T, int R, bool VEC>
 __global__ void __launch_bounds__(256) k_ff_rows(int M, int K, int F, int act, const T* __restrict__ X, long long ldx,
                                                  const T* __restrict__ W, long long ldw, const float* __restrict__ bias,
@@ -890,13 +904,20 @@ __global__ void __launch_bounds__(256) k_ff_rows(int M, int K, int F, int act, c
     const T *wg = W + (size_t)f * ldw, *wu = W + (size_t)(F + f) * ldw;
     for (int m0 = 0; m0 < M; m0 += R) {
         float g[R], u[R];
-#pragma unroll
-        for (int r = 0; r < R; ++r) g[r] = u[r] = 0.f;
         if constexpr (VEC) {
+            f2 gg[R], uu[R];  // even and odd columns
+#pragma unroll
+            for (int r = 0; r < R; ++r) gg[r] = uu[r] = 0;
 #pragma unroll 4
             for (int k = lane * 8; k < K; k += 256) {
                 const uint4 a = __ldg(reinterpret_cast<const uint4*>(wg + k)), c = __ldg(reinterpret_cast<const uint4*>(wu + k));
                 const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, cw[4] = {c.x, c.y, c.z, c.w};
+                f2 p[4], q[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    p[j] = mk(Half2<T>::unpack(aw[j]));
+                    q[j] = mk(Half2<T>::unpack(cw[j]));
+                }
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     if (m0 + r >= M) break;
@@ -904,15 +925,21 @@ __global__ void __launch_bounds__(256) k_ff_rows(int M, int K, int F, int act, c
                     const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const float2 p = Half2<T>::unpack(aw[j]), q = Half2<T>::unpack(cw[j]), y = Half2<T>::unpack(xw[j]);
-                        g[r] = fmaf(p.x, y.x, g[r]);
-                        g[r] = fmaf(p.y, y.y, g[r]);
-                        u[r] = fmaf(q.x, y.x, u[r]);
-                        u[r] = fmaf(q.y, y.y, u[r]);
+                        const f2 y = mk(Half2<T>::unpack(xw[j]));
+                        gg[r] = fma(p[j], y, gg[r]);
+                        uu[r] = fma(q[j], y, uu[r]);
                     }
                 }
             }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float2 x = un(gg[r]), y = un(uu[r]);
+                g[r] = x.x + x.y;
+                u[r] = y.x + y.y;
+            }
         } else {
+#pragma unroll
+            for (int r = 0; r < R; ++r) g[r] = u[r] = 0.f;
 #pragma unroll 4
             for (int k = lane; k < K; k += 32) {
                 const float p = Half2<T>::f(wg[k]), q = Half2<T>::f(wu[k]);

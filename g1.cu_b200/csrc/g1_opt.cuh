@@ -249,7 +249,7 @@ __device__ __forceinline__ double norm_chunks(const Args& A, const Entry* tab) {
 __device__ __forceinline__ float clip_factor(const Args& A, double total, bool write) {
     const double norm = sqrt(total);
     if (write) *A.norm = (float)norm;
-    const double c = A.max_norm / (norm + 1e-6);
+    const double c = isinf(A.max_norm) ? 1.0 : A.max_norm / (norm + 1e-6);  // no limit: not inf / inf
     return c > 1.0 ? 1.f : (float)c;  // a NaN norm stays NaN, as in torch
 }
 

@@ -454,7 +454,9 @@ class _GatedFF(torch.autograd.Function):
 
 def gated_ff(x, w, b=None, act="silu"):
     """gated_ff_device with gradients.  w may be fp32 beside 16-bit rows: it is rounded to their type for the
-    products, and its gradient comes back in fp32.  The forward pass keeps only its inputs."""
+    products, and its gradient comes back in fp32.  The forward pass keeps only its inputs (and copies of those whose
+    rows are not on 16-byte boundaries).  In a captured backward pass the graphs of eager passes over the same leaves have to
+    be gone first, as for any torch operator; gated_ff_backward_device has no such tie."""
     if w.dtype not in (x.dtype, torch.float32):
         raise G1Error("the weights must be fp32 or of the rows' type")
     return _GatedFF.apply(x, w, b, act)
@@ -570,14 +572,23 @@ def _ptrs(tensors):
     return _array(ctypes.c_void_p, list(map(_T.data_ptr, tensors)))
 
 
+def _types(grads):
+    kinds = {g.dtype for g in grads}
+    codes = [_GRAD_TYPE[kinds.pop()]] * len(grads) if len(kinds) == 1 else [_GRAD_TYPE[g.dtype] for g in grads]
+    return _array(ctypes.c_int, codes)
+
+
 def clip_grad_norm_device(grads, max_norm):
     """The global 2-norm over all tensors of `grads` (a tensor or an iterable of fp32 / bf16 / fp16 CUDA tensors; the
     types may differ), and grads *= min(1, max_norm / (norm + 1e-6)) in place (g1_clip_grad_norm), on torch's
     current stream.  Returns the norm before clipping as a CUDA fp32 scalar; nothing synchronises.  The
-    squares are summed in fp64 in a fixed order.  A norm that is NaN or infinite scales as in
-    torch.nn.utils.clip_grad_norm_.  Tensors of one call may not share memory."""
+    squares are summed in fp64 in a fixed order.  max_norm inf: nothing is scaled; otherwise a norm that is NaN or
+    infinite scales as in torch.nn.utils.clip_grad_norm_.  It takes gradients, not the parameters that hold
+    them.  Tensors of one call may not share memory."""
     lib = load_library()
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    if nn.Parameter in set(map(type, grads)):
+        raise G1Error("clip_grad_norm_device takes the gradients, not the parameters")
     dev = _cuda_list(grads, "gradients", _GRAD_TYPE)
     if dev is None:
         _require_gpu()
@@ -587,7 +598,7 @@ def clip_grad_norm_device(grads, max_norm):
     size = lib.g1_opt_workspace(n)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
     with _on(dev):
-        rc = lib.g1_clip_grad_norm(n, _ptrs(grads), _array(ctypes.c_int, [_GRAD_TYPE[g.dtype] for g in grads]),
+        rc = lib.g1_clip_grad_norm(n, _ptrs(grads), _types(grads),
                                    _array(ctypes.c_longlong, list(map(_T.numel, grads))), max_norm, norm.data_ptr(),
                                    ws.data_ptr(), size, _stream_of(dev))
     if rc:

@@ -204,8 +204,8 @@ int g1_gated_ff_status(void);
  * lists are HOST arrays of n DEVICE pointers / values, read during the call only: grads[i] holds counts[i] numbers of
  * types[i] (0 fp32, 1 bf16, 2 fp16), one after another; p, m, v fp32.  Tensors of length 0 are skipped.  Tensors of
  * one call may not share memory.
- *   norm (fp32 [1], DEVICE) <- sqrt(sum of all squares), summed in fp64; c = min(1, max_norm / (norm + 1e-6));
- *   a norm that is NaN or infinite goes through that formula as it does in torch
+ *   norm (fp32 [1], DEVICE) <- sqrt(sum of all squares), summed in fp64; c = min(1, max_norm / (norm + 1e-6)), 1 for
+ *   max_norm inf; a norm that is NaN or infinite goes through that formula as it does in torch
  *   g1_clip_grad_norm  grads *= c in place
  *   g1_clip_adam       one Adam step (decoupled weight decay) of p with the gradients times c, which stay as they
  *                      were; steps (DEVICE int64 [n]) counts each tensor's steps and is advanced by the call, so a

@@ -292,6 +292,94 @@ def test_streams_and_graphs():
     assert torch.equal(h, g1env.gated_ff_device(x, w, b))
 
 
+FIRST = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch, g1env
+x = torch.randn(300, 100, device="cuda").bfloat16()
+w = torch.randn(80, 100, device="cuda").bfloat16()
+dh = torch.randn(300, 40, device="cuda").bfloat16()
+p = torch.nn.Parameter(torch.randn(700000, device="cuda"))
+q = torch.nn.Parameter(torch.randn(70, device="cuda"))
+opt, small = g1env.ClipAdam([p], max_norm=0.5), g1env.ClipAdam([q], max_norm=0.5)
+gp, gq = torch.randn_like(p), torch.randn_like(q)
+graph = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(graph):
+    h = g1env.gated_ff_device(x, w)
+    one = g1env.gated_ff_device(x[:1], w)
+    d = g1env.gated_ff_backward_device(dh, x, w)
+    opt.step([gp]), small.step([gq])
+    n = g1env.clip_grad_norm_device([gp.clone()], 0.5)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(h, g1env.gated_ff_device(x, w)) and torch.equal(one, g1env.gated_ff_device(x[:1], w))
+assert all(torch.equal(a, b) for a, b in zip(d, g1env.gated_ff_backward_device(dh, x, w)))
+assert opt.steps.item() == small.steps.item() == 1 and abs(n.item() - gp.double().norm().item()) < 1e-3
+print("FIRST OK")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture():
+    import os
+    import subprocess
+    import sys
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "g1.cu_b200")
+    r = subprocess.run([sys.executable, "-c", FIRST, pkg], capture_output=True, text=True, timeout=200)
+    assert r.returncode == 0 and "FIRST OK" in r.stdout, r.stdout + r.stderr
+
+
+def test_two_threads_at_once():
+    """Two host threads, each on a stream of its own: the same bits as one after the other."""
+    import threading
+
+    import g1env
+    data = [_make(700 + 300 * i, 96 + 8 * i, 120, B16, True, seed=20 + i) for i in range(2)]
+    want = [[g1env.gated_ff_device(x, w, b), *g1env.gated_ff_backward_device(dh, x, w, b)] for x, w, b, dh in data]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        x, w, b, dh = data[i]
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got = [g1env.gated_ff_device(x, w, b), *g1env.gated_ff_backward_device(dh, x, w, b)]
+                if not all(torch.equal(p, q) for p, q in zip(got, want[i])):
+                    bad.append(i)
+        s.synchronize()
+
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in ts]
+    [t.join() for t in ts]
+    assert not bad
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 numbers in x, h and z: the last rows are where they belong."""
+    import g1env
+    M, K, F = 2_200_000, 1024, 1000
+    free, _ = torch.cuda.mem_get_info()
+    if free < 60e9:
+        pytest.skip("needs 60 GB")
+    g = _gen(1)
+    w = (torch.randn(2 * F, K, device="cuda", generator=g) / 32).to(B16)
+    rows = torch.randn(256, K, device="cuda", generator=g).to(B16)
+    dr = torch.randn(256, F, device="cuda", generator=g).to(B16)
+    x = torch.zeros(M, K, device="cuda", dtype=B16)
+    dh = torch.zeros(M, F, device="cuda", dtype=B16)
+    x[-256:] = rows
+    dh[-256:] = dr
+    h = g1env.gated_ff_device(x, w)
+    assert torch.equal(h[-256:], g1env.gated_ff_device(rows, w)) and not h[:-256].any()
+    dx, dw, db = g1env.gated_ff_backward_device(dh, x, w)
+    a, bw, c = g1env.gated_ff_backward_device(dr, rows, w)
+    assert torch.equal(dx[-256:], a) and not dx[:-256].any()
+    # the same terms, added up in other groups
+    assert bool(((dw.double() - bw.double()).abs() <= 2 * HALF[B16] * bw.double().abs() + 1e-3).all())
+    assert bool(((db - c).abs() <= 1e-4 * (1 + c.abs())).all())
+
+
 def test_refusals():
     import g1env
     x, w, b, dh = _make(4, 16, 8, B16, True, seed=1)

@@ -50,6 +50,7 @@ LISTS = [
     ([1 << 18], [F]),                       # the largest of the one-cluster path
     ([(1 << 18) + 1], [H]),                 # the smallest beyond it
     ([13] * 48 + [400000], [B] * 49),       # a table in the workspace
+    ([5] * 60 + [0], [B, H, F, H] * 15 + [F]),  # one for the one-cluster path
     (list(range(1, 1101)), [F, B, H] * 366 + [F, B]),  # three table launches
     ([30000001, 5], [B, F]),                # long chunks
 ]
@@ -120,6 +121,17 @@ def test_clip_non_finite_as_torch(value, n):
     assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got), torch.isinf(want))
     assert torch.equal(torch.isnan(a), torch.isnan(p.grad))
     assert not torch.nan_to_num(a).any() and not torch.nan_to_num(p.grad).any()
+
+
+def test_no_limit_with_infinite_gradients():
+    """max_norm inf clips nothing: an infinite gradient stays its own tensor's trouble, as in Adam without clipping."""
+    import g1env
+    a = torch.tensor([1.0, float("inf"), 2.0], device="cuda")
+    keep = a.clone()
+    assert g1env.clip_grad_norm_device([a], float("inf")).item() == float("inf") and torch.equal(a, keep)
+    p = torch.nn.Parameter(torch.ones(3, device="cuda"))
+    g1env.ClipAdam([p], lr=0.1).step([a])
+    assert torch.isfinite(p.detach()).tolist() == [True, False, True]
 
 
 def test_clip_deterministic():
@@ -288,6 +300,8 @@ def test_refusals():
     for bad in ([torch.zeros(3)], [c(3).double()], [c(3, 4)[:, :2]], [t, t], [t[:6], t[5:]]):
         with pytest.raises(g1env.G1Error):
             g1env.clip_grad_norm_device(bad, 1.0)
+    with pytest.raises(g1env.G1Error, match="parameters"):
+        g1env.clip_grad_norm_device([torch.nn.Parameter(c(4))], 1.0)
     for norm in (-1.0, float("nan")):
         with pytest.raises(g1env.G1Error):
             g1env.clip_grad_norm_device([t], norm)
