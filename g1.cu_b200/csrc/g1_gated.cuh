@@ -439,7 +439,7 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
 // once; cutting each tile's whole M into runs instead would have the tiles read the same rows at different times.
 template <int MODE>
 struct Tiles {
-    int tile, step;                  // FWD, DZ, DX
+    int tile, step;                  // FWD, DZ, DX: this CTA's first tile, the distance to its next
     int t0, c0, c1, c2, blk;         // DW, DXS: chunks [c0, c1) of tile t0 and [0, c2) of tile t0 + 1 in each block
     // id-th of n CTAs (or groups of CTAs)
     __device__ __forceinline__ Tiles(const Args& P, int id, int n) {
@@ -455,6 +455,17 @@ struct Tiles {
             tile = id;
             step = n;
         }
+    }
+};
+
+// a tile's place, moved on without a division
+struct Place {
+    int m, n, dm, dn, ntn;
+    __device__ __forceinline__ Place(int tile, int step, int ntn_) : m(tile / ntn_), n(tile % ntn_), dm(step / ntn_), dn(step % ntn_), ntn(ntn_) {}
+    __device__ __forceinline__ void next() {
+        m += dm;
+        n += dn;
+        if (n >= ntn) { n -= ntn; ++m; }
     }
 };
 
@@ -654,16 +665,17 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
             constexpr int CH = SC / 8;
             union { uint4 v[CH]; uint32_t w[4 * CH]; } nx;
             float nbg = 0.f, nbu = 0.f;
-            auto ask = [&](int tile, int cc) {
-                if (!PAIR || tile >= ntiles) return;
-                const int col = (tile % ntn) * TN + part * CW + cc;
+            Place here(W.tile, W.step, ntn);
+            auto ask = [&](const Place& at, int cc) {
+                if (!PAIR || at.m >= ntm) return;
+                const int col = at.n * TN + part * CW + cc;
                 nbg = nbu = 0.f;
                 if (P.bias && lane < SC && col + lane < P.N) {
                     nbg = __ldg(P.bias + col + lane);
                     nbu = __ldg(P.bias + P.F + col + lane);
                 }
                 if (MODE == DZ) {
-                    const int row0 = ((tile / ntn) * CG + rank) * BM + 32 * q;
+                    const int row0 = (at.m * CG + rank) * BM + 32 * q;
                     const T* dh = (const T*)P.dh;
                     if (P.vec) {
                         const int ch = lane % CH;
@@ -686,13 +698,17 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                     }
                 }
             };
-            ask(W.tile, 0);
+            ask(here, 0);
             for (int tile = W.tile; tile < ntiles; tile += W.step) {
                 if (!wait(&S.tfull[acc], accph)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;");
-                const int row0 = ((tile / ntn) * CG + rank) * BM + 32 * q;
+                const int row0 = (here.m * CG + rank) * BM + 32 * q, col0 = here.n * TN + part * CW;
+                Place then = here;
+                then.next();
                 const uint32_t t0 = tl + acc * BN + part * CW;
-                // hands the accumulator back once this warp has read its last columns of it
+                // hands the accumulator back once this warp has read its last columns of it.  Nothing but those reads has
+                // to be over by then: a release at cluster scope would wait for the rows written before as well (22 % of
+                // the epilogue's time at K = 104)
                 bool held = true;
                 auto release = [&]() {
                     asm volatile("tcgen05.fence::before_thread_sync;");
@@ -701,14 +717,14 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                         if (CG == 1)
                             asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s32(&S.tempty[acc])) : "memory");
                         else
-                            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(acc ? tempty1 : tempty0)
+                            asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(acc ? tempty1 : tempty0)
                                          : "memory");
                     }
                     held = false;
                 };
 #pragma unroll 1
                 for (int cc = 0; cc < CW; cc += SC) {
-                    const int col = (tile % ntn) * TN + part * CW + cc;
+                    const int col = col0 + cc;
                     const bool some = col < P.N;  // the same for the whole warp
                     if (some && PAIR) {
                         if (lane < SC) { sb[0][lane] = nbg; sb[1][lane] = nbu; }
@@ -726,8 +742,8 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                         }
                         __syncwarp();
                     }
-                    if (cc + SC < CW) ask(tile, cc + SC);
-                    else ask(tile + W.step, 0);
+                    if (cc + SC < CW) ask(here, cc + SC);
+                    else ask(then, 0);
                     if (!some) continue;
 #pragma unroll 1
                     for (int s = 0; s < SC; s += 16) {
@@ -788,6 +804,7 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                     __syncwarp();
                 }
                 if (held) release();  // columns behind the last one
+                here = then;
                 if (++acc == 2) { acc = 0; accph ^= 1u; }
             }
         }
