@@ -266,6 +266,7 @@ constexpr int smem_bytes() { return (int)sizeof(Smem<MODE, BN, CG>) + 1024; }
 // A warp's 32 rows x SC columns go to and from global memory through its buffer, so that neighbouring lanes touch
 // neighbouring addresses (one row a lane would touch 32 lines with each access).  In the buffer the 16-byte groups of a
 // row are permuted so that a column group over 8 rows, and neighbouring groups, lie in different banks.
+// (8 rows further down the permutation is the same: an address moves on by a constant.)
 template <int SC>
 __device__ __forceinline__ int at(int r, int group) {
     return SC == 32 ? r * 64 + ((group ^ ((r >> 1) & 3)) << 4) : r * 32 + ((group ^ ((r >> 2) & 1)) << 4);
@@ -275,14 +276,20 @@ template <class T, int SC>
 __device__ __forceinline__ void rows_out(const uint8_t* buf, T* m, long long ld, int row0, int M, int col, int N, bool vec,
                                          int lane) {
     if (vec) {
-        constexpr int CH = SC / 8;
-        const int ch = lane % CH;
+        constexpr int CH = SC / 8, RS = 32 / CH;
+        const int ch = lane % CH, r = lane / CH;
+        T* dst = m + (size_t)(row0 + r) * ld + col + 8 * ch;
+        const uint8_t* src = buf + at<SC>(r, ch);
+        const bool inside = col + 8 * ch < N;
+        if (row0 + 32 <= M && col + SC <= N) {  // the whole piece
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const int r = lane / CH + i * (32 / CH);
-            if (row0 + r < M && col + 8 * ch < N)
-                *reinterpret_cast<uint4*>(m + (size_t)(row0 + r) * ld + col + 8 * ch) =
-                    *reinterpret_cast<const uint4*>(buf + at<SC>(r, ch));
+            for (int i = 0; i < CH; ++i, dst += RS * ld)
+                *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src + i * RS * SC * 2);
+        } else {
+#pragma unroll
+            for (int i = 0; i < CH; ++i, dst += RS * ld)
+                if (row0 + r + i * RS < M && inside)
+                    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src + i * RS * SC * 2);
         }
     } else {
         const int c = lane % SC;
@@ -328,9 +335,10 @@ __device__ __forceinline__ void dz16(const uint32_t (&rg)[2][8], const uint32_t 
         const int c = s0 + 8 * k + 2 * (lane & 3);
         const f2 bg = *reinterpret_cast<const f2*>(&sb[0][c]), bu = *reinterpret_cast<const f2*>(&sb[1][c]);
         f2 sg = 0, su = 0;
+        const int off0 = at<SC>(lane >> 2, s0 / 8 + k) + (lane & 3) * 4;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int off = at<SC>((lane >> 2) + 8 * i, s0 / 8 + k) + (lane & 3) * 4;
+            const int off = off0 + i * 8 * SC * 2;
             uint32_t* word = reinterpret_cast<uint32_t*>(buf + off);
             const f2 dh = mk(Half2<T>::unpack(*word));
             f2 a, d;
@@ -678,13 +686,17 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                     const int row0 = (at.m * CG + rank) * BM + 32 * q;
                     const T* dh = (const T*)P.dh;
                     if (P.vec) {
-                        const int ch = lane % CH;
+                        constexpr int RS = 32 / CH;
+                        const int ch = lane % CH, r = row0 + lane / CH;
+                        const T* src = dh + (size_t)r * P.F + col + 8 * ch;
+                        if (row0 + 32 <= P.M && col + SC <= P.N) {  // the whole piece
 #pragma unroll
-                        for (int i = 0; i < CH; ++i) {
-                            const int r = row0 + lane / CH + i * (32 / CH);
-                            nx.v[i] = r < P.M && col + 8 * ch < P.N
-                                          ? __ldcs(reinterpret_cast<const uint4*>(dh + (size_t)r * P.F + col + 8 * ch))
-                                          : make_uint4(0, 0, 0, 0);
+                            for (int i = 0; i < CH; ++i, src += (size_t)RS * P.F) nx.v[i] = __ldcs(reinterpret_cast<const uint4*>(src));
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < CH; ++i, src += (size_t)RS * P.F)
+                                nx.v[i] = r + i * RS < P.M && col + 8 * ch < P.N ? __ldcs(reinterpret_cast<const uint4*>(src))
+                                                                                 : make_uint4(0, 0, 0, 0);
                         }
                     } else {  // one number a lane and access, two packed
                         const uint16_t* d16 = reinterpret_cast<const uint16_t*>(dh);
@@ -732,7 +744,7 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                             if (P.vec) {
 #pragma unroll
                                 for (int i = 0; i < CH; ++i)
-                                    *reinterpret_cast<uint4*>(buf + at<SC>(lane / CH + i * (32 / CH), lane % CH)) = nx.v[i];
+                                    *reinterpret_cast<uint4*>(buf + at<SC>(lane / CH, lane % CH) + i * (32 / CH) * SC * 2) = nx.v[i];
                             } else {
 #pragma unroll
                                 for (int i = 0; i < SC; ++i)
