@@ -655,9 +655,8 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
         } else {
             uint32_t acc = 0, accph = 0;
             uint8_t* buf = S.buf[warp - 2][0];
-            uint8_t* buf2 = S.buf[warp - 2][C::BUFS - 1];
+            uint8_t* buf2 = buf + (C::BUFS - 1) * 32 * SC * 2;
             float(*sb)[32] = S.bias[PAIR ? warp - 2 : 0];
-            const uint32_t tempty0 = CG == 1 ? 0 : at_leader(s32(&S.tempty[0])), tempty1 = CG == 1 ? 0 : at_leader(s32(&S.tempty[1]));
             // column (counted from a 16-column step's first) that this lane's sums are of, in its 8-column half
             const int mycol = 2 * (lane & 3) + ((lane >> 3) & 1);
             float* mydb = MODE == DZ && P.db && !(lane & 4) ? P.db + ((size_t)blockIdx.x * 4 + q) * 2 * P.F + (lane & 16 ? P.F : 0)
@@ -715,8 +714,6 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                 if (!wait(&S.tfull[acc], accph)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;");
                 const int row0 = (here.m * CG + rank) * BM + 32 * q, col0 = here.n * TN + part * CW;
-                Place then = here;
-                then.next();
                 const uint32_t t0 = tl + acc * BN + part * CW;
                 // hands the accumulator back once this warp has read its last columns of it.  Nothing but those reads has
                 // to be over by then: a release at cluster scope would wait for the rows written before as well (22 % of
@@ -729,7 +726,7 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                         if (CG == 1)
                             asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s32(&S.tempty[acc])) : "memory");
                         else
-                            asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(acc ? tempty1 : tempty0)
+                            asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(at_leader(s32(&S.tempty[acc])))
                                          : "memory");
                     }
                     held = false;
@@ -754,8 +751,13 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                         }
                         __syncwarp();
                     }
-                    if (cc + SC < CW) ask(here, cc + SC);
-                    else ask(then, 0);
+                    if (cc + SC < CW) {
+                        ask(here, cc + SC);
+                    } else {
+                        Place then = here;
+                        then.next();
+                        ask(then, 0);
+                    }
                     if (!some) continue;
 #pragma unroll 1
                     for (int s = 0; s < SC; s += 16) {
@@ -816,7 +818,7 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                     __syncwarp();
                 }
                 if (held) release();  // columns behind the last one
-                here = then;
+                here.next();
                 if (++acc == 2) { acc = 0; accph ^= 1u; }
             }
         }
