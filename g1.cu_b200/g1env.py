@@ -10,6 +10,7 @@ there is no CPU fallback.
 import contextlib
 import ctypes
 import os
+from array import array
 
 import numpy as np
 import torch
@@ -443,13 +444,20 @@ class _GatedFF(torch.autograd.Function):
         return h
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
-        x, w, b = ctx.saved_tensors  # notices a change made since
-        lib, dev, b2, F, t, code, operands, w_dtype = ctx.call
-        with _on(dev):
-            dx, dw, db = _ff_backward(lib, dev, dh, x, b2, F, t, code, operands, ctx.needs_input_grad, w_dtype)
-        return dx, dw, db if db is None or b.dtype == torch.float32 else db.to(b.dtype), None
+        # once_differentiable costs 6 us a call; only a backward pass that is itself recorded needs it
+        return _gated_ff_once(ctx, dh) if torch.is_grad_enabled() else _gated_ff_back(ctx, dh)
+
+
+def _gated_ff_back(ctx, dh):
+    x, w, b = ctx.saved_tensors  # notices a change made since
+    lib, dev, b2, F, t, code, operands, w_dtype = ctx.call
+    with _on(dev):
+        dx, dw, db = _ff_backward(lib, dev, dh, x, b2, F, t, code, operands, ctx.needs_input_grad, w_dtype)
+    return dx, dw, db if db is None or b.dtype == torch.float32 else db.to(b.dtype), None
+
+
+_gated_ff_once = torch.autograd.function.once_differentiable(_gated_ff_back)
 
 
 def gated_ff(x, w, b=None, act="silu"):
@@ -550,32 +558,34 @@ _T = torch.Tensor
 
 
 def _cuda_list(tensors, what, types):
-    """Checks a list of dense CUDA tensors of those types on one device; their device, None for an empty list."""
+    """Checks a list of dense CUDA tensors of those types on one device; their device (None for an empty list) and types."""
     where = set(map(_T.get_device, tensors))
     if -1 in where:
         raise G1Error(f"{what} must be CUDA tensors")
     if len(where) > 1:
         raise G1Error(f"{what} must be on one device")
-    for t in {t.dtype for t in tensors}:
+    kinds = {t.dtype for t in tensors}
+    for t in kinds:
         if t not in types:
             raise G1Error(f"{what} must be {' / '.join(str(x)[6:] for x in types)}, not {str(t)[6:]}")
     if not all(map(_T.is_contiguous, tensors)) and not all(map(_dense, tensors)):
         raise G1Error(f"{what} must fill their memory without gaps (use .contiguous())")
-    return tensors[0].device if tensors else None
-
-
-def _array(ctype, values):
-    return (ctype * len(values))(*values)
+    return (tensors[0].device if tensors else None), kinds
 
 
 def _ptrs(tensors):
-    return _array(ctypes.c_void_p, list(map(_T.data_ptr, tensors)))
+    return array("Q", map(_T.data_ptr, tensors))
 
 
-def _types(grads):
-    kinds = {g.dtype for g in grads}
-    codes = [_GRAD_TYPE[kinds.pop()]] * len(grads) if len(kinds) == 1 else [_GRAD_TYPE[g.dtype] for g in grads]
-    return _array(ctypes.c_int, codes)
+def _types(grads, kinds):
+    if len(kinds) == 1:
+        return array("i", [_GRAD_TYPE[t] for t in kinds]) * len(grads)
+    return array("i", [_GRAD_TYPE[g.dtype] for g in grads])
+
+
+def _at(a):
+    """where an array's values lie: NULL for an empty one; the array has to live as long as the address is used"""
+    return a.buffer_info()[0] if a else None
 
 
 def clip_grad_norm_device(grads, max_norm):
@@ -589,7 +599,7 @@ def clip_grad_norm_device(grads, max_norm):
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     if nn.Parameter in set(map(type, grads)):
         raise G1Error("clip_grad_norm_device takes the gradients, not the parameters")
-    dev = _cuda_list(grads, "gradients", _GRAD_TYPE)
+    dev, kinds = _cuda_list(grads, "gradients", _GRAD_TYPE)
     if dev is None:
         _require_gpu()
         dev = torch.device("cuda", torch.cuda.current_device())
@@ -597,10 +607,10 @@ def clip_grad_norm_device(grads, max_norm):
     norm = torch.empty((), dtype=torch.float32, device=dev)
     size = lib.g1_opt_workspace(n)
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    ptrs, types, counts = _ptrs(grads), _types(grads, kinds), array("q", map(_T.numel, grads))
     with _on(dev):
-        rc = lib.g1_clip_grad_norm(n, _ptrs(grads), _types(grads),
-                                   _array(ctypes.c_longlong, list(map(_T.numel, grads))), max_norm, norm.data_ptr(),
-                                   ws.data_ptr(), size, _stream_of(dev))
+        rc = lib.g1_clip_grad_norm(n, _at(ptrs), _at(types), _at(counts), max_norm, norm.data_ptr(), ws.data_ptr(), size,
+                                   _stream_of(dev))
     if rc:
         _check()
     torch.autograd.graph.increment_version(grads)
@@ -628,7 +638,7 @@ class ClipAdam:
         self.params = list(params)
         if not self.params:
             raise G1Error("no parameters")
-        self.device = _cuda_list(self.params, "parameters", (torch.float32,))
+        self.device = _cuda_list(self.params, "parameters", (torch.float32,))[0]
         self.lr, self.betas, self.eps = lr, (float(betas[0]), float(betas[1])), float(eps)
         self.max_norm, self.weight_decay = float(max_norm), float(weight_decay)
         like = lambda: [torch.zeros_like(p, requires_grad=False) for p in self.params]
@@ -677,15 +687,15 @@ class ClipAdam:
                     raise G1Error("gradients must be CUDA tensors")
                 grads[i] = torch.empty_like(p, dtype=g.dtype, requires_grad=False).copy_(g.detach())
         there = grads if have == () else [g for g in grads if g is not None]
-        if not set(map(_T.get_device, there)) <= self._where or not {g.dtype for g in there} <= _GRAD_TYPE.keys():
+        kinds = {g.dtype for g in there}
+        if not set(map(_T.get_device, there)) <= self._where or not kinds <= _GRAD_TYPE.keys():
             raise G1Error("gradients must be fp32, bf16 or fp16 on their parameters' device")
         if len(there) == n:
-            ptrs, types, counts = list(map(_T.data_ptr, grads)), [_GRAD_TYPE[g.dtype] for g in grads], self._counts
-            moved = params
+            ptrs, types, counts, moved = _ptrs(grads), _types(grads, kinds), array("q", self._counts), params
         else:
-            ptrs = [None if g is None else g.data_ptr() for g in grads]
-            types = [0 if g is None else _GRAD_TYPE[g.dtype] for g in grads]
-            counts = [0 if g is None else c for g, c in zip(grads, self._counts)]
+            ptrs = array("Q", [0 if g is None else g.data_ptr() for g in grads])
+            types = array("i", [0 if g is None else _GRAD_TYPE[g.dtype] for g in grads])
+            counts = array("q", [0 if g is None else c for g, c in zip(grads, self._counts)])
             moved = [p for p, g in zip(params, grads) if g is not None]
         norm = torch.empty((), dtype=torch.float32, device=dev)
         size = lib.g1_opt_workspace(n)
@@ -695,11 +705,11 @@ class ClipAdam:
             if not (lr.device == dev and lr.dtype == torch.float32 and lr.numel() == 1):
                 raise G1Error("a tensor lr must be one fp32 number on the parameters' device")
             lr, lr_dev = 0.0, lr.data_ptr()
+        p, m, v = _ptrs(params), _ptrs(self.exp_avg), _ptrs(self.exp_avg_sq)
         with _on(dev):
-            rc = lib.g1_clip_adam(n, _array(ctypes.c_void_p, ptrs), _array(ctypes.c_int, types), _ptrs(params),
-                                  _ptrs(self.exp_avg), _ptrs(self.exp_avg_sq), _array(ctypes.c_longlong, counts),
-                                  self.steps.data_ptr(), self.max_norm, lr, lr_dev, self.betas[0], self.betas[1], self.eps,
-                                  self.weight_decay, norm.data_ptr(), ws.data_ptr(), size, _stream_of(dev))
+            rc = lib.g1_clip_adam(n, _at(ptrs), _at(types), _at(p), _at(m), _at(v), _at(counts), self.steps.data_ptr(),
+                                  self.max_norm, lr, lr_dev, self.betas[0], self.betas[1], self.eps, self.weight_decay,
+                                  norm.data_ptr(), ws.data_ptr(), size, _stream_of(dev))
         if rc:
             _check()
         torch.autograd.graph.increment_version(moved + self._state)
