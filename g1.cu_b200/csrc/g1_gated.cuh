@@ -86,9 +86,9 @@ struct Args {
     int vec;                     // rows of the output and of dh are 16-byte aligned
 };
 
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, uint32_t limit = g1gemm::SPIN) {
     const uint32_t a = s32(bar);
-    for (uint32_t it = 0; it < g1gemm::SPIN; ++it) {
+    for (uint32_t it = 0; it < limit; ++it) {
         uint32_t done;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
@@ -1009,6 +1009,15 @@ __global__ void __launch_bounds__(256) k_ff_rows(int M, int K, int F, int act, c
     }
 }
 
+// a wait that runs out: on a barrier that nothing arrives at, with no copy or MMA in flight
+__global__ void __launch_bounds__(32) k_wait_probe(uint32_t limit) {
+    __shared__ uint64_t bar;
+    if (threadIdx.x == 0) {
+        asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(s32(&bar)));
+        if (!wait(&bar, 0u, limit)) atomicExch(&g_err, 1);
+    }
+}
+
 // ------------------------------------------------------------------ host side
 static bool map2d(CUtensorMap* m, int type, const void* base, long long cols, long long rows, long long ld, int box_rows) {
     EncodeTiledFn f = encode_fn();
@@ -1382,6 +1391,13 @@ int g1_gated_ff_backward(int M, int K, int F, int type, int act, const void* dh,
     }
     if (e != cudaSuccess) { set_error((int)e, "g1_gated_ff_backward", cudaGetErrorString(e)); return -1; }
     return 0;
+}
+
+// Test entry (not part of the public header): a wait with a limit of `limit` tries that runs out and says so
+// (g1_gated_ff_status).  Returns the CUDA status.
+int g1_gated_ff_test_wait(unsigned limit, void* stream) {
+    g1ff::k_wait_probe<<<1, 32, 0, (cudaStream_t)stream>>>(limit);
+    return (int)cudaGetLastError();
 }
 
 int g1_gated_ff_status(void) {

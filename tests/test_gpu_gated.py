@@ -329,6 +329,21 @@ def test_first_calls_of_a_process_inside_a_capture():
     assert r.returncode == 0 and "FIRST OK" in r.stdout, r.stdout + r.stderr
 
 
+def test_a_wait_that_runs_out_is_reported():
+    """Failure detection without a GPU fault: a bounded wait on a barrier that nothing arrives at."""
+    import ctypes
+
+    import g1env
+    lib = g1env.load_library()
+    lib.g1_gated_ff_test_wait.argtypes = [ctypes.c_uint, ctypes.c_void_p]
+    assert g1env.gated_ff_status() == 0
+    assert lib.g1_gated_ff_test_wait(4096, None) == 0
+    assert g1env.gated_ff_status() == 1 and g1env.gated_ff_status() == 0
+    x, w, b, dh = _make(300, 64, 40, B16, True, seed=8)
+    first = g1env.gated_ff_device(x, w, b)
+    assert torch.equal(first, g1env.gated_ff_device(x, w, b)) and g1env.gated_ff_status() == 0
+
+
 def test_two_threads_at_once():
     """Two host threads, each on a stream of its own: the same bits as one after the other."""
     import threading
