@@ -54,18 +54,21 @@ namespace g1ff {
 using g1gemm::s32;
 
 constexpr int BM = 128, BK = 64;  // rows of A a CTA, chunk of the sum
-enum { FWD = 0, DZ = 1, DX = 2, DW = 3, DXS = 4 };  // DXS: DX with its sum cut, as DW's
+// DXS: DX with its sum cut, as DW's; DZU: DZ for rows of dh that do not start on 16-byte boundaries
+enum { FWD = 0, DZ = 1, DX = 2, DW = 3, DXS = 4, DZU = 5 };
 // CG: CTAs that work on a tile together (cta_group); BN: columns of B a tile
 template <int MODE, int BN, int CG>
 struct Cfg {
-    static constexpr bool PAIR = MODE == FWD || MODE == DZ;
+    static constexpr bool Z = MODE == DZ || MODE == DZU, PAIR = MODE == FWD || Z;
     static constexpr int TN = PAIR ? BN / 2 : BN;                  // output columns a tile
     static constexpr int PARTS = TN >= 64 ? 4 : TN / 16;           // epilogue warps a TMEM lane quarter
     static constexpr int EPI = 4 * PARTS, NTH = 64 + 32 * EPI;
     static constexpr int CW = TN / PARTS, SC = CW >= 32 ? 32 : 16; // columns a warp, and a step of it
     static constexpr int NB = BN / CG;                             // columns of B in this CTA's memory
-    static constexpr int STAGES = MODE == DZ ? 4 : MODE == FWD ? 5 : MODE == DX ? 6 : 7;
-    static constexpr int BUFS = MODE == DZ ? 2 : MODE == DW || MODE == DXS ? 0 : 1;
+    static constexpr int STAGES = Z ? 4 : MODE == FWD ? 5 : MODE == DX ? 6 : 7;
+    // bytes of a warp's buffer: 32 rows x SC columns; DZ two of them and 32 x 16 more
+    static constexpr int PIECE = 32 * SC * 2, AHEAD = MODE == DZ ? 2 : 1;
+    static constexpr int BUF = MODE == DW || MODE == DXS ? 16 : AHEAD * PIECE + (Z ? 1024 : 0);
     static constexpr int STAGE_BYTES = (BM + NB) * BK * 2;
 };
 constexpr int DW_BLOCK = 64;  // chunks (of 64 rows) that the CTAs of DW walk together
@@ -257,8 +260,8 @@ struct Smem {
     using C = Cfg<MODE, BN, CG>;
     uint8_t a[C::STAGES][BM * BK * 2];
     uint8_t b[C::STAGES][C::NB * BK * 2];
-    uint8_t buf[C::BUFS ? C::EPI : 1][C::BUFS ? C::BUFS : 1][C::BUFS ? 32 * C::SC * 2 : 16];
-    float bias[C::PAIR ? C::EPI : 1][2][32];
+    uint8_t buf[C::BUF > 16 ? C::EPI : 1][C::BUF];
+    float bias[C::PAIR ? C::EPI : 1][C::AHEAD][2][32];
     uint64_t full[C::STAGES], empty[C::STAGES], tfull[2], tempty[2];
     uint32_t tslot;
     volatile int stop;  // a wait of this CTA ran out
@@ -328,31 +331,54 @@ __device__ __forceinline__ void fwd8(const uint32_t* rg, const uint32_t* ru, con
         *reinterpret_cast<float2*>(h + j) = un(mul(a, add(acc2(ru + j), mk(bu[j], bu[j + 1]))));
     }
 }
-// z of 32 rows x 16 columns: dh in `buf` is replaced by dg, du goes to `buf2`; the column sums over the rows to s[k][]:
-// columns 8 k + 2 (l % 4), + 1 of dg, then of du
+// 32 rows x 8 columns of 16-bit numbers as four 8 x 8 matrices: lane l gives the address of row l and holds
+// w[i] = (row 8 i + l / 4, columns 2 (l % 4), + 1)
+__device__ __forceinline__ void load_rows(uint32_t addr, uint32_t* w) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void store_rows(uint32_t addr, const uint32_t* w) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                 : "memory");
+}
+
+// 16 or 4 bytes to shared memory behind the threads' back, zeros where ok is false
+__device__ __forceinline__ void fetch16(uint32_t dst, const void* src, bool ok) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void fetch4(uint32_t dst, const void* src, bool ok) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
+}
+
+// z of 32 rows x 16 columns, the s0-th on: dh in `buf` is replaced by dg, du goes to `buf2` (16 columns); the column
+// sums over the rows to sum[k][]: columns 8 k + 2 (l % 4), + 1 of dg, then of du
 template <class T, int ACT, int SC>
 __device__ __forceinline__ void dz16(const uint32_t (&rg)[2][8], const uint32_t (&ru)[2][8], const float (*sb)[32], int s0,
-                                     uint8_t* buf, uint8_t* buf2, float (&sum)[2][4], int lane) {
+                                     uint32_t buf, uint32_t buf2, float (&sum)[2][4], int lane) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const int c = s0 + 8 * k + 2 * (lane & 3);
         const f2 bg = *reinterpret_cast<const f2*>(&sb[0][c]), bu = *reinterpret_cast<const f2*>(&sb[1][c]);
         f2 sg = 0, su = 0;
-        const int off0 = at<SC>(lane >> 2, s0 / 8 + k) + (lane & 3) * 4;
+        const uint32_t place = buf + at<SC>(lane, s0 / 8 + k);
+        uint32_t w[4], v[4];
+        load_rows(place, w);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int off = off0 + i * 8 * SC * 2;
-            uint32_t* word = reinterpret_cast<uint32_t*>(buf + off);
-            const f2 dh = mk(Half2<T>::unpack(*word));
+            const f2 dh = mk(Half2<T>::unpack(w[i]));
             f2 a, d;
             act2<ACT, true>(add(acc2(&rg[i / 2][4 * k + 2 * (i & 1)]), bg), a, d);
             const f2 dg = mul(mul(dh, add(acc2(&ru[i / 2][4 * k + 2 * (i & 1)]), bu)), d), du = mul(dh, a);
             const float2 x = un(dg), y = un(du);
-            *word = Half2<T>::pack(x.x, x.y);
-            *reinterpret_cast<uint32_t*>(buf2 + off) = Half2<T>::pack(y.x, y.y);
+            w[i] = Half2<T>::pack(x.x, x.y);
+            v[i] = Half2<T>::pack(y.x, y.y);
             sg = add(sg, dg);
             su = add(su, du);
         }
+        store_rows(place, w);
+        store_rows(buf2 + at<16>(lane, k), v);
         const float2 x = un(sg), y = un(su);
         sum[k][0] = x.x; sum[k][1] = x.y; sum[k][2] = y.x; sum[k][3] = y.y;
     }
@@ -485,7 +511,7 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
     using C = Cfg<MODE, BN, CG>;
     extern __shared__ uint8_t smem_raw[];
     auto& S = *reinterpret_cast<Smem<MODE, BN, CG>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    constexpr bool A_MN = MODE == DW, B_MN = MODE >= DX, PAIR = C::PAIR, CUT = MODE == DW || MODE == DXS;
+    constexpr bool A_MN = MODE == DW, PAIR = C::PAIR, Z = C::Z, B_MN = !PAIR, CUT = MODE == DW || MODE == DXS;
     constexpr int TN = C::TN, STAGES = C::STAGES, NB = C::NB;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = CG == 1 ? 0 : (int)cta_rank();
@@ -657,62 +683,59 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
             }
         } else {
             uint32_t acc = 0, accph = 0;
-            uint8_t* buf = S.buf[warp - 2][0];
-            uint8_t* buf2 = buf + (C::BUFS - 1) * 32 * SC * 2;
-            float(*sb)[32] = S.bias[PAIR ? warp - 2 : 0];
-            // column (counted from a 16-column step's first) that this lane's sums are of, in its 8-column half
+            constexpr int CH = SC / 8, RS = 32 / CH, AHEAD = C::AHEAD;  // 16-byte groups a row, rows a step of rows_out
+            uint8_t* buf = S.buf[warp - 2];
+            float(*bias)[2][32] = S.bias[PAIR ? warp - 2 : 0];
+            // Z: column (counted from a 16-column step's first) that this lane's sums are of, in its 8-column half
             const int mycol = 2 * (lane & 3) + ((lane >> 3) & 1);
-            float* mydb = MODE == DZ && P.db && !(lane & 4) ? P.db + ((size_t)blockIdx.x * 4 + q) * 2 * P.F + (lane & 16 ? P.F : 0)
-                                                            : nullptr;
-            if (MODE == DZ && mydb) {
+            float* mydb = Z && P.db && !(lane & 4) ? P.db + ((size_t)blockIdx.x * 4 + q) * 2 * P.F + (lane & 16 ? P.F : 0) : nullptr;
+            if (Z && mydb) {
                 // the sums start at 0; the additions below are the same thread's, so they come after
                 for (int c = part * CW + mycol; c < P.N; c += TN)
                     for (int e = 0; e < CW; e += 8)
                         if (c + e < P.N) mydb[c + e] = 0.f;
             }
-            // the bias (a column a lane) and dh (as rows_out lays out its accesses) of a step are asked for one step ahead,
-            // a tile's first before the wait for its products
-            constexpr int CH = SC / 8;
-            union { uint4 v[CH]; uint32_t w[4 * CH]; } nx;
+            // The bias (a column a lane) and dh of a step are asked for one step ahead, a tile's first before the wait for its
+            // products: in DZ by asynchronous copies into the other of two buffers, else through registers (which DZ has
+            // none to spare of: with dh in them it spilled, 171 us instead of 117 at 65536 x 104 x 1024).
+            uint32_t nx[MODE == DZU ? SC / 2 : 1];
             float nbg = 0.f, nbu = 0.f;
-            Place here(W.tile, W.step, ntn);
-            auto ask = [&](const Place& at, int cc) {
-                if (!PAIR || at.m >= ntm) return;
-                const int col = at.n * TN + part * CW + cc;
-                nbg = nbu = 0.f;
-                if (P.bias && lane < SC && col + lane < P.N) {
-                    nbg = __ldg(P.bias + col + lane);
-                    nbu = __ldg(P.bias + P.F + col + lane);
-                }
+            auto ask = [&](const Place& to, int cc, int into) {
+                if (!PAIR || to.m >= ntm) return;
+                const int col = to.n * TN + part * CW + cc, row0 = (to.m * CG + rank) * BM + 32 * q;
+                const bool b = P.bias && lane < SC && col + lane < P.N;
+                const float* bg = P.bias + col + lane;
                 if (MODE == DZ) {
-                    const int row0 = (at.m * CG + rank) * BM + 32 * q;
-                    const T* dh = (const T*)P.dh;
-                    if (P.vec) {
-                        constexpr int RS = 32 / CH;
-                        const int ch = lane % CH, r = row0 + lane / CH;
-                        const T* src = dh + (size_t)r * P.F + col + 8 * ch;
-                        if (row0 + 32 <= P.M && col + SC <= P.N) {  // the whole piece
+                    if (lane < SC) {
+                        fetch4(s32(&bias[into][0][lane]), b ? (const void*)bg : P.dh, b);
+                        fetch4(s32(&bias[into][1][lane]), b ? (const void*)(bg + P.F) : P.dh, b);
+                    }
+                    const int ch = lane % CH, r = row0 + lane / CH;
+                    const T* src = (const T*)P.dh + (size_t)r * P.F + col + 8 * ch;
+                    const uint32_t dst = s32(buf) + into * C::PIECE + at<SC>(lane / CH, ch);
 #pragma unroll
-                            for (int i = 0; i < CH; ++i, src += (size_t)RS * P.F) nx.v[i] = __ldcs(reinterpret_cast<const uint4*>(src));
-                        } else {
+                    for (int i = 0; i < CH; ++i, src += (size_t)RS * P.F) {
+                        const bool ok = r + i * RS < P.M && col + 8 * ch < P.N;
+                        fetch16(dst + i * RS * SC * 2, ok ? (const void*)src : P.dh, ok);
+                    }
+                } else {
+                    nbg = b ? __ldg(bg) : 0.f;
+                    nbu = b ? __ldg(bg + P.F) : 0.f;
+                }
+                if (MODE == DZU) {  // one number a lane and access, two packed
+                    const uint16_t* d16 = reinterpret_cast<const uint16_t*>(P.dh);
+                    const int c = col + lane % SC;
 #pragma unroll
-                            for (int i = 0; i < CH; ++i, src += (size_t)RS * P.F)
-                                nx.v[i] = r + i * RS < P.M && col + 8 * ch < P.N ? __ldcs(reinterpret_cast<const uint4*>(src))
-                                                                                 : make_uint4(0, 0, 0, 0);
-                        }
-                    } else {  // one number a lane and access, two packed
-                        const uint16_t* d16 = reinterpret_cast<const uint16_t*>(dh);
-                        const int c = col + lane % SC;
-#pragma unroll
-                        for (int i = 0; i < SC; ++i) {
-                            const int r = row0 + lane / SC + i * (32 / SC);
-                            const uint32_t x = r < P.M && c < P.N ? d16[(size_t)r * P.F + c] : 0;
-                            nx.w[i / 2] = i & 1 ? nx.w[i / 2] | (x << 16) : x;
-                        }
+                    for (int i = 0; i < SC; ++i) {
+                        const int r = row0 + lane / SC + i * (32 / SC);
+                        const uint32_t x = r < P.M && c < P.N ? d16[(size_t)r * P.F + c] : 0;
+                        nx[MODE == DZU ? i / 2 : 0] = i & 1 ? nx[MODE == DZU ? i / 2 : 0] | (x << 16) : x;
                     }
                 }
             };
-            ask(here, 0);
+            Place here(W.tile, W.step, ntn);
+            int cur = 0;
+            ask(here, 0, 0);
             for (int tile = W.tile; tile < ntiles; tile += W.step) {
                 if (!wait(&S.tfull[acc], accph)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;");
@@ -738,33 +761,32 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                 for (int cc = 0; cc < CW; cc += SC) {
                     const int col = col0 + cc;
                     const bool some = col < P.N;  // the same for the whole warp
-                    if (some && PAIR) {
-                        if (lane < SC) { sb[0][lane] = nbg; sb[1][lane] = nbu; }
-                        if (MODE == DZ) {
-                            if (P.vec) {
+                    if (MODE == DZ) asm volatile("cp.async.wait_all;" ::: "memory");
+                    if (MODE != DZ && PAIR && some) {
+                        if (lane < SC) { bias[0][0][lane] = nbg; bias[0][1][lane] = nbu; }
+                        if (MODE == DZU) {
 #pragma unroll
-                                for (int i = 0; i < CH; ++i)
-                                    *reinterpret_cast<uint4*>(buf + at<SC>(lane / CH, lane % CH) + i * (32 / CH) * SC * 2) = nx.v[i];
-                            } else {
-#pragma unroll
-                                for (int i = 0; i < SC; ++i)
-                                    *reinterpret_cast<uint16_t*>(buf + at<SC>(lane / SC + i * (32 / SC), lane % SC / 8) + lane % 8 * 2) =
-                                        (uint16_t)(nx.w[i / 2] >> (16 * (i & 1)));
-                            }
+                            for (int i = 0; i < SC; ++i)
+                                *reinterpret_cast<uint16_t*>(buf + at<SC>(lane / SC + i * (32 / SC), lane % SC / 8) + lane % 8 * 2) =
+                                    (uint16_t)(nx[MODE == DZU ? i / 2 : 0] >> (16 * (i & 1)));
                         }
-                        __syncwarp();
                     }
+                    __syncwarp();
                     if (cc + SC < CW) {
-                        ask(here, cc + SC);
+                        ask(here, cc + SC, cur ^ 1);
                     } else {
                         Place then = here;
                         then.next();
-                        ask(then, 0);
+                        ask(then, 0, cur ^ 1);
                     }
+                    uint8_t* mine = buf + (AHEAD == 2 ? cur * C::PIECE : 0);
+                    const float(*sb)[32] = bias[AHEAD == 2 ? cur : 0];
+                    cur ^= 1;
                     if (!some) continue;
 #pragma unroll 1
                     for (int s = 0; s < SC; s += 16) {
-                        if (MODE == DZ) {
+                        if (Z) {
+                            uint8_t* du = buf + AHEAD * C::PIECE;
                             uint32_t rg[2][8], ru[2][8];
                             tmem_ld16x16(t0 + cc + s, rg[0]);
                             tmem_ld16x16(t0 + (16u << 16) + cc + s, rg[1]);
@@ -773,10 +795,10 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                             if (cc + s + 16 == CW) release();
                             float sum[2][4];
-                            if (P.act == 0) dz16<T, 0, SC>(rg, ru, sb, s, buf, buf2, sum, lane);
-                            else if (P.act == 1) dz16<T, 1, SC>(rg, ru, sb, s, buf, buf2, sum, lane);
-                            else if (P.act == 2) dz16<T, 2, SC>(rg, ru, sb, s, buf, buf2, sum, lane);
-                            else dz16<T, 3, SC>(rg, ru, sb, s, buf, buf2, sum, lane);
+                            if (P.act == 0) dz16<T, 0, SC>(rg, ru, sb, s, s32(mine), s32(du), sum, lane);
+                            else if (P.act == 1) dz16<T, 1, SC>(rg, ru, sb, s, s32(mine), s32(du), sum, lane);
+                            else if (P.act == 2) dz16<T, 2, SC>(rg, ru, sb, s, s32(mine), s32(du), sum, lane);
+                            else dz16<T, 3, SC>(rg, ru, sb, s, s32(mine), s32(du), sum, lane);
                             if (P.db) {  // rows behind the last one have dh = 0
 #pragma unroll
                                 for (int k = 0; k < 2; ++k) {
@@ -786,6 +808,10 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                                     if (mydb && c < P.N) atomicAdd(mydb + c, v);
                                 }
                             }
+                            __syncwarp();
+                            // z's rows are padded to whole 16-byte groups
+                            rows_out<T, 16>(du, (T*)P.out + P.ldo / 2, P.ldo, row0, P.M, col + s, P.N, true, lane);
+                            __syncwarp();
                             continue;
                         }
                         uint32_t r[16];
@@ -811,19 +837,18 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
 #pragma unroll
                                 for (int j = 0; j < 8; ++j) h[j] = __uint_as_float(r[e + j]);
                             }
-                            *reinterpret_cast<uint4*>(buf + at<SC>(lane, (s + e) / 8)) = pack8<T>(h);
+                            *reinterpret_cast<uint4*>(mine + at<SC>(lane, (s + e) / 8)) = pack8<T>(h);
                         }
                     }
                     __syncwarp();
-                    // z's rows are padded to whole 16-byte groups
-                    rows_out<T, SC>(buf, (T*)P.out, P.ldo, row0, P.M, col, P.N, MODE == DZ || P.vec, lane);
-                    if (MODE == DZ) rows_out<T, SC>(buf2, (T*)P.out + P.ldo / 2, P.ldo, row0, P.M, col, P.N, true, lane);
+                    rows_out<T, SC>(mine, (T*)P.out, P.ldo, row0, P.M, col, P.N, Z || P.vec, lane);
                     __syncwarp();
                 }
                 if (held) release();  // columns behind the last one
                 here.next();
                 if (++acc == 2) { acc = 0; accph ^= 1u; }
             }
+            if (MODE == DZ) asm volatile("cp.async.wait_all;" ::: "memory");  // nothing in flight, even after a wait that ran out
         }
     }
     if (!ok) {
@@ -1258,7 +1283,7 @@ static cudaError_t backward(Call c, const Plan& L, const void* dh, void* dx, voi
         P.dh = dh;
         P.vec = c.F % 8 == 0 && ((uintptr_t)dh & 15) == 0;
         P.db = db ? (float*)(c.ws + L.db) : nullptr;
-        e = pair_tiles<T, DZ>(c, P, &ctas);
+        e = P.vec ? pair_tiles<T, DZ>(c, P, &ctas) : pair_tiles<T, DZU>(c, P, &ctas);
         if (e != cudaSuccess) return e;
     }
     const float* db_part = (const float*)(c.ws + L.db);
