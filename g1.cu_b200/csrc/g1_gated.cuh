@@ -32,15 +32,16 @@
 // What bounds it: the products.  A chunk's 32 KB a CTA are written to and read from shared memory in the 512 cycles of its
 // MMAs, close to the 128 bytes a cycle that it has (tensor pipe 74 % active in DX, 56 % in DZ, whose epilogue moves
 // dh, dg and du through shared memory as well); under the power cap of a long step the clock gives way first.  Below
-// K = 500 or so the epilogues do: 2.7 us a 128 x 128 tile and CTA in FWD, 6.0 us in DZ.
+// K = 500 or so the epilogues do: 2.7 us a 128 x 128 tile and CTA in FWD, 4.2 us in DZ.
 // Measured on one B200 (graph replays; percent of the measured 1659 TFLOP/s):
 //   forward 32768 x 1024 x 1024              100 us   1370 TFLOP/s   83 %
-//   forward and backward 524288 x 1024 x 512 3.7 to 4.0 ms, by box: FWD 0.80, DZ 0.95, DX 0.83, DW 0.87 each by itself;
+//   forward and backward 524288 x 1024 x 512 3.7 to 4.0 ms, by box: FWD 0.80, DZ 0.93, DX 0.82, DW 0.84 each by itself;
 //                                            869 TFLOP/s of the 12MKF that cannot be avoided, 1158 of the 16MKF run
-//   forward 65536 x 104 x 1024               79 to 96 us; 151 MB
+//   forward 65536 x 104 x 1024               81 us, its DZ 117 us by itself; 151 and 418 MB
 //   forward 1 x 1024 x 1024                  2.0 us   2.1 TB/s from L2: latency
 // Steps: 128-row tiles by single CTAs 117 us and 4.57 ms; pairs of CTAs 109 us and 4.29 ms; coalesced epilogue with
-// two-number arithmetic 101 us and 3.9 ms; accumulators handed back before the stores, no bank conflicts, no spills 3.7 ms.
+// two-number arithmetic 101 us and 3.9 ms; accumulators handed back before the stores, no bank conflicts 3.7 ms; DZ alone from
+// 0.98 to 0.93 ms without spills (at K = 104 from 181 to 117 us).
 // Taken out: the next tile's A fetched to L2 ahead, by the loading thread (115 us, 4.6 ms) or by the second CTA's idle MMA
 // warp (no change); 8 epilogue warps of 64 columns (K = 104: 118 us, 16 warps 88).
 #pragma once
