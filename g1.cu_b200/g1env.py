@@ -629,7 +629,8 @@ class ClipAdam:
 
     step() reads each parameter's .grad, step(grads) a list of fp32 / bf16 / fp16 gradients (None: left alone).
     It returns the norm before clipping as a CUDA scalar; the gradients keep their values.  Nothing
-    synchronises, and a step captured into a CUDA graph counts on at each replay."""
+    synchronises, and a step captured into a CUDA graph counts on at each replay.  lr, betas, eps, max_norm and
+    weight_decay are plain attributes, read at each step (at capture, for a captured one; a tensor lr at each replay)."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, max_norm=float("inf"), weight_decay=0.0,
                  moments=None, steps=0):

@@ -140,7 +140,7 @@ def test_update_with_clipped_adam():
     assert moved > 0 and apart <= 0.05 * moved
 
 
-@pytest.mark.parametrize("flags", [["--gated", "--fused-opt"], ["--fused-opt"]])
+@pytest.mark.parametrize("flags", [["--gated", "--fused-opt"], ["--fused-opt"], ["--config4", "--gated", "--no-eval"]])
 def test_trainer_command(flags):
     r = subprocess.run([sys.executable, os.path.join(ROOT, "g1.cu_b200", "ppo_fused.py"), "2", "64", "--smoke", "--tag=gated_test"]
                        + flags, capture_output=True, text=True, timeout=300)
