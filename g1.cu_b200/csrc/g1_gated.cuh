@@ -1098,13 +1098,16 @@ constexpr int ROWS_MAX = 4;  // rows up to which the forward pass goes by k_ff_r
 
 // Columns of B a tile, for `cols` output columns that B has `per` of for each: 256 on pairs of CTAs (cg 2) where that
 // gives two of three pairs a tile, else 128 or 64 on single ones, the narrower the fewer tiles there are.  Measured, forward:
-// 2048 x 1024 x 1024 (64 pair tiles) 12.0 us on pairs, 15.9 on single CTAs; 1024 x 1024 x 1024 (32) 11.0 and 9.8.
+// 2048 x 1024 x 1024 (64 pair tiles) 12.0 us on pairs, 15.9 on single CTAs; 1024 x 1024 x 1024 (32) 11.0 and 9.8.  Matrices of
+// up to 128 columns on pairs too: backward 65536 x 104 x 1024 233 us, on single CTAs 255.  (Halving the columns of wider
+// ones to fill the last wave does not pay, as a half tile takes as long: forward 20000 x 512 x 512 31.7 us, 21.7 without.)
 struct Shape {
     int bn, cg;
 };
 static Shape tile_shape(int M, int cols, int per, int nsm) {
     auto tiles = [&](int rows, int bn) { return (long long)((M + rows - 1) / rows) * ((cols * per + bn - 1) / bn); };
     if (cols * per > 128 && tiles(2 * BM, 256) * 3 >= nsm) return {256, 2};
+    if (cols * per > 64 && cols * per <= 128 && tiles(2 * BM, 128) * 3 >= nsm) return {128, 2};
     if (cols * per > 64 && tiles(BM, 128) * 2 > nsm) return {128, 1};
     return {64, 1};
 }
@@ -1139,7 +1142,7 @@ static Plan plan(int M, int K, int F, const void* X, long long ldx, const void* 
         L.db = take((long long)nsm * 4 * 2 * F * 4);
         const int nk = (M + BK - 1) / BK;
         // a short sum: small tiles on all SMs, as it is the writing of dW that takes the time
-        L.dw = K <= 64 ? Shape{64, 1} : K <= 128 || nk <= 8 ? Shape{128, 1} : Shape{256, 2};
+        L.dw = K <= 64 ? Shape{64, 1} : K <= 128 || nk <= 8 ? (nk > DW_BLOCK ? Shape{128, 2} : Shape{128, 1}) : Shape{256, 2};
         const int all = nsm / L.dw.cg;
         L.tiles = 2 * ((F + BM - 1) / BM) / L.dw.cg * ((K + L.dw.bn - 1) / L.dw.bn);
         L.passes = (L.tiles + all - 1) / all;
@@ -1211,7 +1214,7 @@ static cudaError_t pair_tiles(const Call& c, Args P, int* ctas) {
     const int groups = (int)std::min<long long>((long long)((c.M + rows - 1) / rows) * ((c.F + tn - 1) / tn), c.nsm / sh.cg);
     *ctas = groups * sh.cg;
     if (sh.bn == 64) return launch<T, MODE, 64, 1>(P, groups, c.st);
-    if (sh.bn == 128) return launch<T, MODE, 128, 1>(P, groups, c.st);
+    if (sh.bn == 128) return sh.cg == 2 ? launch<T, MODE, 128, 2>(P, groups, c.st) : launch<T, MODE, 128, 1>(P, groups, c.st);
     return launch<T, MODE, 256, 2>(P, groups, c.st);
 }
 
@@ -1312,7 +1315,7 @@ static cudaError_t backward(Call c, const Plan& L, const void* dh, void* dx, voi
             const int rows = BM * sh.cg;
             const int groups = (int)std::min<long long>((long long)((c.M + rows - 1) / rows) * ((c.K + sh.bn - 1) / sh.bn), c.nsm / sh.cg);
             e = sh.bn == 64    ? launch<T, DX, 64, 1>(P, groups, c.st)
-                : sh.bn == 128 ? launch<T, DX, 128, 1>(P, groups, c.st)
+                : sh.bn == 128 ? (sh.cg == 2 ? launch<T, DX, 128, 2>(P, groups, c.st) : launch<T, DX, 128, 1>(P, groups, c.st))
                                : launch<T, DX, 256, 2>(P, groups, c.st);
         }
         if (e != cudaSuccess) return e;
@@ -1325,8 +1328,9 @@ static cudaError_t backward(Call c, const Plan& L, const void* dh, void* dx, voi
         P.M = c.M; P.N = c.K; P.F = c.F;
         P.nk = (c.M + BK - 1) / BK;
         return L.dw.bn == 64    ? dw_passes<T, 64, 1>(c, L, P, dw, dw_type, db_part, db, ctas * 4)
-               : L.dw.bn == 128 ? dw_passes<T, 128, 1>(c, L, P, dw, dw_type, db_part, db, ctas * 4)
-                                : dw_passes<T, 256, 2>(c, L, P, dw, dw_type, db_part, db, ctas * 4);
+               : L.dw.bn == 256 ? dw_passes<T, 256, 2>(c, L, P, dw, dw_type, db_part, db, ctas * 4)
+               : L.dw.cg == 2   ? dw_passes<T, 128, 2>(c, L, P, dw, dw_type, db_part, db, ctas * 4)
+                                : dw_passes<T, 128, 1>(c, L, P, dw, dw_type, db_part, db, ctas * 4);
     }
     if (db) e = sum_tiles<T, T, 64, 1>(c, nullptr, (T*)nullptr, c.F, 0, 0, 1, 1, db_part, db, ctas * 4);
     return e;

@@ -94,7 +94,9 @@ SHAPES = [(1, 1, 1), (1, 8, 8), (3, 17, 5), (128, 64, 128), (129, 65, 129), (2, 
           (64, 1024, 1024), (1000, 1024, 64), (2, 2048, 300), (5000, 40, 24), (777, 264, 501), (20000, 128, 136),
           (8200, 130, 700), (200, 2048, 2048),
           # sums of dx cut over CTAs (few rows, many outputs), on 64 and 128 columns; dw in two passes with cut sums
-          (70, 40, 2500), (100, 104, 2600), (129, 129, 3001), (19000, 2048, 2048)]
+          (70, 40, 2500), (100, 104, 2600), (129, 129, 3001), (19000, 2048, 2048),
+          # narrow matrices on pairs of CTAs
+          (13000, 100, 60), (13001, 520, 40)]
 
 
 @pytest.mark.parametrize("t", [B16, F16], ids=["bf16", "fp16"])
