@@ -359,30 +359,28 @@ def _bytes(x, n):
 
 
 def _ff_forward(lib, dev, x, x2, w, b, F, t, code):
-    """h, and the operands as a backward call takes them: where their rows are not aligned, the copies that this call
-    leaves at the start of its workspace (the last of what is returned)."""
+    """h, and where rows are not aligned the workspace with their copies and how many bytes of it are x's and w's."""
     M, K, px, ldx, pw, ldw = _ff_operands(x2, w)
-    n, ws, copies = 0, None, None
+    nx = nw = n = 0
+    ws = None
     if M > 4 and ((px | pw) & 15 or (ldx | ldw) & 7):
         k8 = (K + 7) & ~7
         nx = (M * k8 * 2 + 255) & ~255 if px & 15 or ldx & 7 else 0
         nw = (F * k8 * 4 + 255) & ~255 if pw & 15 or ldw & 7 else 0
         n = nx + nw
         ws = _bytes(x, n)
-        at = ws.data_ptr()
-        copies = (M, K, at if nx else px, k8 if nx else ldx, at + nx if nw else pw, k8 if nw else ldw)
     h = x.new_empty(x.shape[:-1] + (F,))
     if lib.g1_gated_ff(M, K, F, t, code, px, ldx, pw, ldw, _addr(b), h.data_ptr(), _addr(ws), n, _stream_of(dev)):
         _check()
-    return h, copies or (M, K, px, ldx, pw, ldw), ws
+    return h, ws, nx, nw
 
 
-def _ff_backward(lib, dev, dh, x, b, F, t, code, operands, need, dw_dtype):
+def _ff_backward(lib, dev, dh, x, shape, b, F, t, code, operands, need, dw_dtype):
     M, K, px, ldx, pw, ldw = operands
     n = lib.g1_gated_ff_workspace(M, K, F, px, ldx, pw, ldw, 1)
     ws = _bytes(x, n)
     dh = dh.contiguous()
-    dx = x.new_empty(x.shape) if need[0] else None
+    dx = x.new_empty(shape) if need[0] else None
     dw = x.new_empty((2 * F, K), dtype=dw_dtype) if need[1] else None
     db = x.new_empty(2 * F, dtype=torch.float32) if need[2] else None
     if lib.g1_gated_ff_backward(M, K, F, t, code, dh.data_ptr(), px, ldx, pw, ldw, _addr(b), _addr(dx), _addr(dw),
@@ -421,7 +419,7 @@ def gated_ff_backward_device(dh, x, w, b=None, act="silu", need=(True, True, Tru
     if dh.device != dev or dh.dtype != x.dtype or dh.shape != x.shape[:-1] + (F,):
         raise G1Error("dh must be [..., F] on x's device and of its type")
     with _on(dev):
-        return _ff_backward(lib, dev, dh, x, b, F, t, code, _ff_operands(x2, w), need, dw_dtype)
+        return _ff_backward(lib, dev, dh, x, x.shape, b, F, t, code, _ff_operands(x2, w), need, dw_dtype)
 
 
 def gated_ff_status():
@@ -437,10 +435,9 @@ class _GatedFF(torch.autograd.Function):
         x2, w2, b2, F, t, code = _ff_args(x, w16, b, act)
         dev = x2.device
         with _on(dev):
-            h, operands, ws = _ff_forward(lib, dev, x, x2, w2, b2, F, t, code)
-        ctx.save_for_backward(x, w, b)
-        ctx.call = (lib, dev, b2, F, t, code, operands, w.dtype)
-        ctx.keep = (x2, w2, ws)  # what the operands' addresses are of
+            h, ws, nx, nw = _ff_forward(lib, dev, x, x2, w2, b2, F, t, code)
+        ctx.save_for_backward(x2, w2, b2, ws)
+        ctx.call = (lib, dev, F, t, code, nx, nw, x.shape, w.dtype, None if b is None else b.dtype)
         return h
 
     @staticmethod
@@ -450,11 +447,18 @@ class _GatedFF(torch.autograd.Function):
 
 
 def _gated_ff_back(ctx, dh):
-    x, w, b = ctx.saved_tensors  # notices a change made since
-    lib, dev, b2, F, t, code, operands, w_dtype = ctx.call
+    # notices a change made since; a hook may have put other tensors in their place
+    x2, w2, b2, ws = ctx.saved_tensors
+    lib, dev, F, t, code, nx, nw, shape, w_dtype, b_dtype = ctx.call
+    x2, w2 = _rows(x2), _rows(w2)
+    operands = _ff_operands(x2, w2)
+    if ws is not None:  # the forward pass's copies of unaligned rows
+        M, K, px, ldx, pw, ldw = operands
+        at, k8 = ws.data_ptr(), (K + 7) & ~7
+        operands = (M, K, at if nx else px, k8 if nx else ldx, at + nx if nw else pw, k8 if nw else ldw)
     with _on(dev):
-        dx, dw, db = _ff_backward(lib, dev, dh, x, b2, F, t, code, operands, ctx.needs_input_grad, w_dtype)
-    return dx, dw, db if db is None or b.dtype == torch.float32 else db.to(b.dtype), None
+        dx, dw, db = _ff_backward(lib, dev, dh, x2, shape, b2, F, t, code, operands, ctx.needs_input_grad, w_dtype)
+    return dx, dw, db if db is None or b_dtype == torch.float32 else db.to(b_dtype), None
 
 
 _gated_ff_once = torch.autograd.function.once_differentiable(_gated_ff_back)
@@ -462,9 +466,10 @@ _gated_ff_once = torch.autograd.function.once_differentiable(_gated_ff_back)
 
 def gated_ff(x, w, b=None, act="silu"):
     """gated_ff_device with gradients.  w may be fp32 beside 16-bit rows: it is rounded to their type for the
-    products, and its gradient comes back in fp32.  The forward pass keeps only its inputs (and copies of those whose
-    rows are not on 16-byte boundaries).  In a captured backward pass the graphs of eager passes over the same leaves have to
-    be gone first, as for any torch operator; gated_ff_backward_device has no such tie."""
+    products, and its gradient comes back in fp32.  The forward pass keeps only its inputs as the products take them (w
+    rounded; copies of those whose rows are not on 16-byte boundaries), as saved tensors that hooks and checkpoints see.
+    In a captured backward pass the graphs of eager passes over the same leaves have to be gone first, as for any torch
+    operator; gated_ff_backward_device has no such tie."""
     if w.dtype not in (x.dtype, torch.float32):
         raise G1Error("the weights must be fp32 or of the rows' type")
     return _GatedFF.apply(x, w, b, act)

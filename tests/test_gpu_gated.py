@@ -262,6 +262,46 @@ def test_autograd_shared_weights_and_master_weights():
         torch.autograd.grad(gw.sum(), leaves[1])
 
 
+@pytest.mark.parametrize("K,off", [(48, 0), (45, 0), (48, 1)])
+def test_saved_tensors_go_through_hooks(K, off):
+    """What the forward pass saves is what the backward pass works on: copies that a hook made (of which the originals may
+    change), or those that a checkpoint makes again; and it is let go once the backward pass has been through."""
+    import g1env
+    from torch.utils.checkpoint import checkpoint
+    x, w, b, dh = _make(150, K, 48, B16, True, seed=16)
+    at = torch.empty(150 * K + off, dtype=B16, device="cuda")[off:].view(150, K)  # off 1: not on 16-byte boundaries
+    want = g1env.gated_ff_backward_device(dh, x, w, b)
+    for kind in ("copies", "host", "checkpoint"):
+        wl, bl = w.clone().requires_grad_(), b.clone().requires_grad_()
+        xl = at.copy_(x).detach().requires_grad_()
+        if kind == "checkpoint":
+            h = checkpoint(g1env.gated_ff, xl, wl, bl, use_reentrant=False)
+        else:
+            hooks = (torch.autograd.graph.save_on_cpu(pin_memory=True) if kind == "host"
+                     else torch.autograd.graph.saved_tensors_hooks(torch.clone, lambda t: t))
+            with hooks:
+                h = g1env.gated_ff(xl, wl, bl)
+            torch.cuda.synchronize()
+            with torch.no_grad():
+                at.fill_(float("nan"))
+                wl.fill_(float("nan"))
+                bl.fill_(float("nan"))
+        h.backward(dh)
+        for leaf, g in zip((xl, wl, bl), want):
+            assert torch.equal(leaf.grad, g), kind
+    # a layer's rows between two layers: freed by its backward pass, not with the graph's last name
+    rows = 1 << 16
+    x, w, b, dh = _make(rows, 64, 64, B16, True, seed=17)
+    wl = w.clone().requires_grad_()
+    h = x
+    for _ in range(8):
+        h = g1env.gated_ff(h, wl)
+    mem = torch.cuda.memory_allocated()
+    h.backward(dh)
+    wl.grad = None
+    assert torch.cuda.memory_allocated() <= mem - 7 * rows * 64 * 2
+
+
 def test_streams_and_graphs():
     """Two captured calls with workspaces of their own, replayed in turn on new inputs, and a call on another stream."""
     import g1env
