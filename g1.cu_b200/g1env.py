@@ -658,6 +658,7 @@ class ClipAdam:
                     raise G1Error("moments must be laid out like their parameters")
         self.steps = torch.full((len(self.params),), int(steps), dtype=torch.int64, device=self.device)
         self._counts = [p.numel() for p in self.params]
+        self._shapes = [p.shape for p in self.params]
         self._strides = [p.stride() for p in self.params]
         self._where = {self.device.index}
         self._state = self.exp_avg + self.exp_avg_sq + [self.steps]
@@ -675,14 +676,15 @@ class ClipAdam:
         if len(grads) != n:
             raise G1Error("step takes one gradient (or None) a parameter")
         lib = _lib
-        if (list(map(_T.stride, params)) != self._strides or list(map(_T.numel, params)) != self._counts
+        if (list(map(_T.stride, params)) != self._strides or list(map(_T.size, params)) != self._shapes
                 or set(map(_T.get_device, params)) != self._where or {p.dtype for p in params} != {torch.float32}):
             raise G1Error("a parameter is no longer laid out as it was when the optimiser was made")
         if any(g is None for g in grads):
             have = [i for i, g in enumerate(grads) if g is not None]
         else:
             have = range(n)
-            if list(map(_T.stride, grads)) == self._strides and list(map(_T.numel, grads)) == self._counts:
+            # shapes too: [6, 1] and [2, 3] may share strides (3, 1) and lengths, and only one of them has no gaps
+            if list(map(_T.stride, grads)) == self._strides and list(map(_T.size, grads)) == self._shapes:
                 have = ()  # nothing to look at one by one
         for i in have:
             g, p = grads[i], params[i]

@@ -1,0 +1,67 @@
+"""ClipAdam's host side without a GPU: which gradients reach the library.  The library is a fake that keeps the calls; the
+tensors are on the CPU, so only the checks of device are out of the way."""
+import contextlib
+
+import pytest
+import torch
+
+
+class _Fake:
+    def __init__(self):
+        self.calls = []
+
+    def g1_opt_workspace(self, n):
+        return 64
+
+    def g1_clip_adam(self, n, *args):
+        self.calls.append((n,) + args)
+        return 0
+
+
+@pytest.fixture
+def make(monkeypatch):
+    import g1env
+    fake = _Fake()
+    monkeypatch.setattr(g1env, "_lib", fake)
+    monkeypatch.setattr(g1env, "_require_gpu", lambda: None)
+    monkeypatch.setattr(g1env, "load_library", lambda: fake)
+    monkeypatch.setattr(g1env, "_cuda_list", lambda ts, what, types: (torch.device("cpu"), {t.dtype for t in ts}))
+    monkeypatch.setattr(g1env, "_on", lambda dev: contextlib.nullcontext())
+    monkeypatch.setattr(g1env, "_stream_of", lambda dev: 0)
+
+    def build(params, **kw):
+        opt = g1env.ClipAdam(params, **kw)
+        opt._where = {-1}  # where get_device() says that CPU tensors are
+        return opt, fake
+    return build
+
+
+# shapes of parameter and gradient, and the gradient: equal strides and lengths do not make equal shapes
+def _cases():
+    z = torch.zeros
+    return [((2, 3), z(3, 3)[:, :2]),                             # [3, 2], strides (3, 1)
+            ((2, 3), z(6, 3)[:, :1]),                             # [6, 1], strides (3, 1)
+            ((4, 3), z(9).as_strided((2, 6), (3, 1))),            # overlaps itself: 9 numbers where 12 would be read
+            ((2, 3), z(6)), ((2, 3), z(3, 2)), ((6,), z(2, 3))]
+
+
+@pytest.mark.parametrize("i", range(6))
+def test_gradients_of_other_shapes_are_refused(make, i):
+    import g1env
+    shape, g = _cases()[i]
+    opt, fake = make([torch.nn.Parameter(torch.zeros(shape))])
+    with pytest.raises(g1env.G1Error, match="shapes"):
+        opt.step([g])
+    assert not fake.calls
+    opt.step([torch.zeros(shape)])
+    assert len(fake.calls) == 1 and fake.calls[0][0] == 1
+
+
+def test_parameter_of_another_shape_is_noticed(make):
+    import g1env
+    p = torch.nn.Parameter(torch.zeros(2, 3))
+    opt, fake = make([p])
+    p.data = torch.zeros(3, 3)[:, :2]
+    with pytest.raises(g1env.G1Error, match="laid out"):
+        opt.step([torch.zeros(2, 3)])
+    assert not fake.calls
