@@ -27,6 +27,7 @@
 #include <mutex>
 #include <string>
 
+#include "g1_buffers.h"
 #include "g1_physics.cuh"
 #include "g1_mlp_tc.cuh"
 #include "g1_gemm_tma.cuh"
@@ -1068,6 +1069,17 @@ struct EnvState {
     cudaStream_t stream;                // 0 = legacy default stream (the reference's)
 };
 
+// the env's device error flag, made on first use
+static cudaError_t error_flag(EnvState* E) {
+    if (E->derr) return cudaSuccess;
+    int* p = nullptr;
+    cudaError_t e = cudaMalloc(&p, sizeof(int));
+    if (e == cudaSuccess) e = cudaMemset(p, 0, sizeof(int));
+    if (e == cudaSuccess) E->derr = p;
+    else cudaFree(p);
+    return e;
+}
+
 static std::once_flag g_tab_once[64];
 static int upload_tables(int dev) {
     int rc = 0;
@@ -1255,33 +1267,16 @@ static void rollout_tc(EnvState* E, int H, const float* W, const float* mean, co
             if (!head) { vs += (long long)vin * no + no; vin = E->vhid[l]; }
             if (E->vhid[l] > maxw && !head) maxw = E->vhid[l];
         }
-        if (E->tc_wvb < (size_t)vdw || E->tc_bv < (size_t)vdb || E->tc_hdv < (size_t)N) {
-            cudaFree(E->Wvb); cudaFree(E->Bvf); cudaFree(E->HDv);
-            E->Wvb = nullptr; E->Bvf = nullptr; E->HDv = nullptr; E->tc_wvb = 0; E->tc_bv = 0; E->tc_hdv = 0;
-            CKR(cudaMalloc(&E->Wvb, (size_t)vdw * 2), );
-            CKR(cudaMalloc(&E->Bvf, (size_t)vdb * 4), );
-            CKR(cudaMalloc(&E->HDv, (size_t)N * 32 * 4), );
-            E->tc_wvb = vdw; E->tc_bv = vdb; E->tc_hdv = N;
-        }
+        CKR(grow({{&E->tc_wvb, (size_t)vdw}, {&E->tc_bv, (size_t)vdb}, {&E->tc_hdv, (size_t)N}},
+                 {grow_buf(&E->Wvb, vdw), grow_buf(&E->Bvf, vdb), grow_buf(&E->HDv, (size_t)N * 32)}), );
     }
     // buffers (allocated on first use, kept by the env)
-    if (E->tc_N < (size_t)N || E->tc_w < (size_t)maxw) {
-        cudaFree(E->Xb); cudaFree(E->Hb[0]); cudaFree(E->Hb[1]); cudaFree(E->HD);
-        E->Xb = E->Hb[0] = E->Hb[1] = nullptr; E->HD = nullptr;
-        CKR(cudaMalloc(&E->Xb, (size_t)N * XK * 2), );
-        CKR(cudaMalloc(&E->Hb[0], (size_t)N * maxw * 2), );
-        CKR(cudaMalloc(&E->Hb[1], (size_t)N * maxw * 2), );
-        CKR(cudaMalloc(&E->HD, (size_t)N * 32 * 4), );
-        E->tc_N = N; E->tc_w = maxw;
-    }
-    if (E->tc_wb < (size_t)dw || E->tc_b < (size_t)db) {
-        cudaFree(E->Wb); cudaFree(E->Bf); cudaFree(E->LS);
-        CKR(cudaMalloc(&E->Wb, (size_t)dw * 2), );
-        CKR(cudaMalloc(&E->Bf, (size_t)db * 4), );
-        CKR(cudaMalloc(&E->LS, 32 * 4), );
-        E->tc_wb = dw; E->tc_b = db;
-    }
-    if (!E->derr) { CKR(cudaMalloc(&E->derr, sizeof(int)), ); CKR(cudaMemset(E->derr, 0, sizeof(int)), ); }
+    CKR(grow({{&E->tc_N, (size_t)N}, {&E->tc_w, (size_t)maxw}},
+             {grow_buf(&E->Xb, (size_t)N * XK), grow_buf(&E->Hb[0], (size_t)N * maxw), grow_buf(&E->Hb[1], (size_t)N * maxw),
+              grow_buf(&E->HD, (size_t)N * 32)}), );
+    CKR(grow({{&E->tc_wb, (size_t)dw}, {&E->tc_b, (size_t)db}},
+             {grow_buf(&E->Wb, dw), grow_buf(&E->Bf, db), grow_buf(&E->LS, 32)}), );
+    CKR(error_flag(E), );
     k_repack_bf16<<<240, 256, 0, E->stream>>>(W, E->Wb, E->Bf, E->LS, RP);
     CKR(cudaGetLastError(), );
     if (vnet) {
@@ -1362,10 +1357,7 @@ static int tc_error(EnvState* E) {
 // device flag as the rollout's, read with g1_env_tc_status.  Returns the CUDA status.
 extern "C" int g1_env_test_wait_timeout(void* h, unsigned spin_limit) {
     EnvState* E = (EnvState*)h;
-    if (!E->derr) {
-        CKR(cudaMalloc(&E->derr, sizeof(int)), -1);
-        CKR(cudaMemset(E->derr, 0, sizeof(int)), -1);
-    }
+    CKR(error_flag(E), -1);
     g1tc::k_wait_probe<<<1, 224, 0, E->stream>>>(E->derr, spin_limit);
     cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess) e = cudaStreamSynchronize(E->stream);
@@ -1593,17 +1585,8 @@ static bool prepare_tf(EnvState* E, const float* W, Params& P) {
     RP.srcLS = src + (long long)ACT_DIM * nin + ACT_DIM + nin + 1;
     const size_t img_bytes = ((size_t)dw * 2 + 255) & ~(size_t)255;
     const size_t need = img_bytes + ((size_t)db + 32) * 4;
-    if (need > E->tf_cap) {
-        cudaFree(E->tf_img);
-        E->tf_img = nullptr;
-        E->tf_cap = 0;
-        CKR(cudaMalloc(&E->tf_img, need), false);
-        E->tf_cap = need;
-    }
-    if (!E->derr) {
-        CKR(cudaMalloc(&E->derr, sizeof(int)), false);
-        CKR(cudaMemset(E->derr, 0, sizeof(int)), false);
-    }
+    CKR(grow({{&E->tf_cap, need}}, {grow_buf(&E->tf_img, need)}), false);
+    CKR(error_flag(E), false);
     __nv_bfloat16* img = reinterpret_cast<__nv_bfloat16*>(E->tf_img);
     float* bias = reinterpret_cast<float*>(E->tf_img + img_bytes);
     k_repack_tf<<<148, 256, 0, E->stream>>>(W, img, bias, bias + db, RP);
@@ -1629,12 +1612,7 @@ void g1_rollout(void* h, int H, const float* W, const float* mean, const float* 
         return;
     }
     size_t need = policy_floats(E->nh, E->hid);
-    if (need > E->WT_cap) {
-        cudaFree(E->WT);
-        E->WT = nullptr;
-        CKR(cudaMalloc(&E->WT, need * 4), );
-        E->WT_cap = need;
-    }
+    CKR(grow({{&E->WT_cap, need}}, {grow_buf(&E->WT, need)}), );
     Params P = base_params(E);
     if (tf_eligible(E)) {
         if (!prepare_tf(E, W, P)) return;
