@@ -250,7 +250,9 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t* r) {
 }
 
 // A launch may start while the one before it in the stream ends (programmatic dependent launch): set up, then wait here
-// before the first access to memory that another kernel writes.
+// before the first access to memory that another kernel writes.  The kernel is resident while that one still writes, so it
+// reads by ordinary loads: read-only ones (ld.global.nc, which the compiler also makes of const __restrict__ arguments) want
+// their data to stay as it is for as long as the kernel lives.
 __device__ __forceinline__ void after_previous() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
@@ -720,8 +722,8 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                         fetch16(dst + i * RS * SC * 2, ok ? (const void*)src : P.dh, ok);
                     }
                 } else {
-                    nbg = b ? __ldg(bg) : 0.f;
-                    nbu = b ? __ldg(bg + P.F) : 0.f;
+                    nbg = b ? *bg : 0.f;
+                    nbu = b ? bg[P.F] : 0.f;
                 }
                 if (MODE == DZU) {  // one number a lane and access, two packed
                     const uint16_t* d16 = reinterpret_cast<const uint16_t*>(P.dh);
@@ -955,9 +957,8 @@ __global__ void __launch_bounds__(256) k_pad(PadJob a, PadJob b, int ldd, int n)
 // a lane (VEC; single numbers where rows start anywhere), the rows of X come from L1.  R rows at a time.  Measured in a
 // graph, this and 128-row tiles: 1 x 1024 x 1024 2.1 us and 8.1, 4 rows 5.7 and 8.1 (8 rows took 9.9)
 template <class T, int R, bool VEC>
-__global__ void __launch_bounds__(256) k_ff_rows(int M, int K, int F, int act, const T* __restrict__ X, long long ldx,
-                                                 const T* __restrict__ W, long long ldw, const float* __restrict__ bias,
-                                                 T* __restrict__ h) {
+__global__ void __launch_bounds__(256) k_ff_rows(int M, int K, int F, int act, const T* X, long long ldx, const T* W, long long ldw,
+                                                 const float* bias, T* __restrict__ h) {
     const int f = (blockIdx.x * 256 + threadIdx.x) >> 5, lane = threadIdx.x & 31;
     after_previous();
     if (f >= F) return;
@@ -970,7 +971,7 @@ __global__ void __launch_bounds__(256) k_ff_rows(int M, int K, int F, int act, c
             for (int r = 0; r < R; ++r) gg[r] = uu[r] = 0;
 #pragma unroll 4
             for (int k = lane * 8; k < K; k += 256) {
-                const uint4 a = __ldg(reinterpret_cast<const uint4*>(wg + k)), c = __ldg(reinterpret_cast<const uint4*>(wu + k));
+                const uint4 a = *reinterpret_cast<const uint4*>(wg + k), c = *reinterpret_cast<const uint4*>(wu + k);
                 const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, cw[4] = {c.x, c.y, c.z, c.w};
                 f2 p[4], q[4];
 #pragma unroll
@@ -981,7 +982,7 @@ __global__ void __launch_bounds__(256) k_ff_rows(int M, int K, int F, int act, c
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     if (m0 + r >= M) break;
-                    const uint4 x = __ldg(reinterpret_cast<const uint4*>(X + (m0 + r) * ldx + k));
+                    const uint4 x = *reinterpret_cast<const uint4*>(X + (m0 + r) * ldx + k);
                     const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {

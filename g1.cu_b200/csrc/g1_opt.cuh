@@ -116,7 +116,8 @@ __device__ __forceinline__ long long chunk_of(const Entry& e, long long c, int c
     return lo;
 }
 
-// A launch may start while the one before it in the stream ends: wait here before the first access to memory
+// A launch may start while the one before it in the stream ends: wait here before the first access to memory.  Loads
+// are ordinary ones: data of read-only ones would have to stay as it is for as long as the kernel is resident
 __device__ __forceinline__ void after_previous() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;");
@@ -175,8 +176,8 @@ __device__ __forceinline__ void adam1(float g, float& p, float& m, float& v, con
 }
 
 template <class T>
-__device__ __forceinline__ void adam(const T* __restrict__ g, float* __restrict__ p, float* __restrict__ m,
-                                     float* __restrict__ v, int cnt, const Coef& k) {
+__device__ __forceinline__ void adam(const T* g, float* __restrict__ p, float* __restrict__ m, float* __restrict__ v, int cnt,
+                                     const Coef& k) {
     const int tid = threadIdx.x, nt = blockDim.x;
     int head = head_of(p, cnt);
     // 4-wide where all four pointers reach their boundary after the same number of elements
