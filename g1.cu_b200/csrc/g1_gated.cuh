@@ -106,6 +106,9 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, uint32_t li
     return false;
 }
 
+// for a whole warp: all lanes go on or none, as what follows (tcgen05.ld, ldmatrix) is for whole warps
+__device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); }
+
 // MN-major SWIZZLE_128B descriptor of 64 x 64 boxes 8 KB apart: LBO = the next 64 along M or N, SBO = the next 8
 // along the sum (8 rows of 128 bytes)
 __device__ __forceinline__ uint64_t desc_mn(uint32_t saddr) {
@@ -657,7 +660,7 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                 if (!have) continue;
                 // all of the CTA's products lie before this: as long as 64 other waits, or until one of those ran out
                 ok = false;
-                for (int i = 0; i < 64 && !ok && !S.stop; ++i) ok = wait(&S.tfull[a], 0);
+                for (int i = 0; i < 64 && !ok && !__any_sync(0xffffffffu, S.stop); ++i) ok = wait_all(&S.tfull[a], 0);
                 if (!ok) break;
                 asm volatile("tcgen05.fence::after_thread_sync;");
                 const size_t row = ((size_t)(blockIdx.x / CG + W.t0 + a) * CG + rank) * BM + 32 * q + lane;
@@ -670,13 +673,15 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                     tmem_ld16(tl + a * BN + part * CW + cc, r);
                     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                     if (MODE == DW && P.direct) {
-                        if (f >= P.F) continue;
-                        float v[16];
+                        if (f < P.F) {
+                            float v[16];
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
-                        const size_t at0 = (size_t)(up ? P.F + f : f) * P.N + k0 + cc;
-                        if (P.out32) store16((float*)P.out + at0, v, P.N - k0 - cc, P.vec);
-                        else store16((T*)P.out + at0, v, P.N - k0 - cc, P.vec);
+                            for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+                            const size_t at0 = (size_t)(up ? P.F + f : f) * P.N + k0 + cc;
+                            if (P.out32) store16((float*)P.out + at0, v, P.N - k0 - cc, P.vec);
+                            else store16((T*)P.out + at0, v, P.N - k0 - cc, P.vec);
+                        }
+                        __syncwarp();  // the next columns are read by whole warps
                         continue;
                     }
 #pragma unroll
@@ -740,7 +745,7 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
             int cur = 0;
             ask(here, 0, 0);
             for (int tile = W.tile; tile < ntiles; tile += W.step) {
-                if (!wait(&S.tfull[acc], accph)) { ok = false; break; }
+                if (!wait_all(&S.tfull[acc], accph)) { ok = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;");
                 const int row0 = (here.m * CG + rank) * BM + 32 * q, col0 = here.n * TN + part * CW;
                 const uint32_t t0 = tl + acc * BN + part * CW;
