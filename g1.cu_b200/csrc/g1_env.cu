@@ -1057,7 +1057,7 @@ struct EnvState {
     int prec;                           // 0: fp32 in-kernel policy, 1: bf16 tensor-core policy
     __nv_bfloat16 *Xb, *Hb[2], *Wb;     // large-policy activations and weights
     float *Bf, *LS, *HD;
-    int* derr;
+    int* derr;                          // a wait of this env's kernels ran out (see k_take_flag)
     size_t tc_N, tc_w, tc_wb, tc_b;
     int vnh, vhid[MAX_HIDDEN];          // separate value network (bf16 path), vnh = 0: shared trunk
     __nv_bfloat16* Wvb;
@@ -1073,8 +1073,8 @@ struct EnvState {
 static cudaError_t error_flag(EnvState* E) {
     if (E->derr) return cudaSuccess;
     int* p = nullptr;
-    cudaError_t e = cudaMalloc(&p, sizeof(int));
-    if (e == cudaSuccess) e = cudaMemset(p, 0, sizeof(int));
+    cudaError_t e = cudaMalloc(&p, 2 * sizeof(int));
+    if (e == cudaSuccess) e = cudaMemset(p, 0, 2 * sizeof(int));
     if (e == cudaSuccess) E->derr = p;
     else cudaFree(p);
     return e;
@@ -1291,7 +1291,7 @@ static void rollout_tc(EnvState* E, int H, const float* W, const float* mean, co
     const dim3 oblk(32, 8);
     const int ogrid = (N + 7) / 8;
     auto layer = [&](int width, int k, const __nv_bfloat16* in, const __nv_bfloat16* Wl, const float* bl, __nv_bfloat16* out) {
-        return gated ? g1ff::policy_layer(N, k, width, E->act, in, Wl, bl, out, E->sm_count, E->stream)
+        return gated ? g1ff::policy_layer(N, k, width, E->act, in, Wl, bl, out, E->sm_count, E->derr, E->stream)
                      : dense_tc(N, width, k, in, k, Wl, bl, E->act, nullptr, 0, out, width, E->derr, E->stream);
     };
     auto policy = [&](int row, uint64_t tick) -> bool {
@@ -1337,19 +1337,20 @@ static void rollout_tc(EnvState* E, int H, const float* W, const float* mean, co
     E->tick += (uint64_t)H;
 }
 
-// Device error flag of the tensor-core path (a timed-out MMA wait); read and cleared.
+// derr: the flag, and the value that it had when it was last taken
+static __global__ void k_take_flag(int* derr) { derr[1] = atomicExch(derr, 0); }
+
+// Device error flag of the env's tensor-core path (a timed-out MMA wait), read and cleared behind the work of its stream.
 static int tc_error(EnvState* E) {
     if (!E->derr) return 0;
-    int herr = 0;
-    if (cudaMemcpy(&herr, E->derr, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) return -1;
-    if (herr) cudaMemset(E->derr, 0, sizeof(int));
-    if (E->act >= 2) {  // the gated layers' own flag, on the env's device
-        int dev = E->device;
-        if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(E->device) != cudaSuccess) return -1;
-        herr |= g1_gated_ff_status();
-        cudaSetDevice(dev);
-    }
-    return herr;
+    int dev = E->device, herr = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(E->device) != cudaSuccess) return -1;
+    k_take_flag<<<1, 1, 0, E->stream>>>(E->derr);
+    cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) e = cudaMemcpyAsync(&herr, E->derr + 1, sizeof(int), cudaMemcpyDeviceToHost, E->stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(E->stream);
+    cudaSetDevice(dev);
+    return e == cudaSuccess ? herr : -1;
 }
 
 // Test entry (not part of the public header): runs k_wait_probe on the env's stream with a

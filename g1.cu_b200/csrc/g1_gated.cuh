@@ -26,8 +26,8 @@
 //
 // Operands come by TMA (128-byte swizzle, zero fill past the edges, no multicast) in chunks of 64 along the sum, four to seven
 // stages; one thread issues the loads, one the MMAs, up to sixteen warps run the epilogue of a tile while the
-// next one accumulates in the other half of tensor memory.  Every wait is bounded; one that runs out sets g_err
-// (g1_gated_ff_status), and the kernel ends with garbage in its outputs.
+// next one accumulates in the other half of tensor memory.  Every wait is bounded; one that runs out sets a flag, an env's own
+// (g1_env_tc_status) or the device's for all other calls (g1_gated_ff_status), and the kernel ends with garbage in its outputs.
 //
 // What bounds it: the products.  A chunk's 32 KB a CTA are written to and read from shared memory in the 512 cycles of its
 // MMAs, close to the 128 bytes a cycle that it has (tensor pipe 74 % active in DX, 56 % in DZ, whose epilogue moves
@@ -74,7 +74,8 @@ struct Cfg {
 };
 constexpr int DW_BLOCK = 64;  // chunks (of 64 rows) that the CTAs of DW walk together
 
-__device__ int g_err;  // a wait ran out
+__device__ int g_err;    // a wait of a call that brings no flag of its own ran out
+__device__ int g_taken;  // g_err as k_take_err found it
 
 struct Args {
     CUtensorMap a0, a1, b0, b1;  // gate / up halves where they differ
@@ -88,6 +89,7 @@ struct Args {
     int tile0, ntp, blk;         // DW, DXS: the pass's tiles, chunks a block (see Tiles)
     int direct, out32;           // DW: every CTA has the whole sum of its tile: dW itself is written, in fp32 or 16 bits
     int vec;                     // rows of the output and of dh are 16-byte aligned
+    int* err;                    // the flag of a wait that ran out; null: g_err
 };
 
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, uint32_t limit = g1gemm::SPIN) {
@@ -861,7 +863,7 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
     }
     if (!ok) {
         S.stop = 1;
-        atomicExch(&g_err, 1);
+        atomicExch(P.err ? P.err : &g_err, 1);
         if (warp == 0)  // give loads in flight 0.1 s to land
             for (int i = 0; i < 100; ++i) __nanosleep(1000000);
     }
@@ -1050,6 +1052,8 @@ __global__ void __launch_bounds__(32) k_wait_probe(uint32_t limit) {
     }
 }
 
+__global__ void k_take_err() { g_taken = atomicExch(&g_err, 0); }
+
 // ------------------------------------------------------------------ host side
 static bool map2d(CUtensorMap* m, int type, const void* base, long long cols, long long rows, long long ld, int box_rows) {
     EncodeTiledFn f = encode_fn();
@@ -1188,6 +1192,7 @@ struct Call {
     uint8_t* ws;
     cudaStream_t st;
     int nsm;
+    int* err;  // forward: the flag of a wait that runs out, or null for the device's
 };
 
 static cudaError_t operands(Call& c, const Plan& L) {
@@ -1215,7 +1220,7 @@ static cudaError_t pair_tiles(const Call& c, Args P, int* ctas) {
     if (!map2d(&P.a0, c.type, c.X, c.K, c.M, c.ldx, BM) || !map2d(&P.b0, c.type, c.W, c.K, c.F, c.ldw, tn) ||
         !map2d(&P.b1, c.type, (const T*)c.W + c.F * c.ldw, c.K, c.F, c.ldw, tn))
         return cudaErrorInvalidValue;
-    P.M = c.M; P.N = c.F; P.F = c.F; P.act = c.act; P.bias = c.b;
+    P.M = c.M; P.N = c.F; P.F = c.F; P.act = c.act; P.bias = c.b; P.err = c.err;
     P.nk = (c.K + BK - 1) / BK;
     const int groups = (int)std::min<long long>((long long)((c.M + rows - 1) / rows) * ((c.F + tn - 1) / tn), c.nsm / sh.cg);
     *ctas = groups * sh.cg;
@@ -1342,11 +1347,12 @@ static cudaError_t backward(Call c, const Plan& L, const void* dh, void* dx, voi
     return e;
 }
 
-// a gated layer of the wide policies' rollout: bf16, rows and weights on 16-byte boundaries (K a multiple of 8)
+// a gated layer of the wide policies' rollout: bf16, rows and weights on 16-byte boundaries (K a multiple of 8); err: the
+// env's flag
 static cudaError_t policy_layer(int M, int K, int F, int act, const __nv_bfloat16* X, const __nv_bfloat16* W, const float* b,
-                                __nv_bfloat16* h, int nsm, cudaStream_t st) {
+                                __nv_bfloat16* h, int nsm, int* err, cudaStream_t st) {
     if (needs_pad(X, K) || needs_pad(W, K)) return cudaErrorInvalidValue;
-    const Call c = {M, K, F, 1, act, X, K, W, K, b, nullptr, st, nsm};
+    const Call c = {M, K, F, 1, act, X, K, W, K, b, nullptr, st, nsm, err};
     return forward<__nv_bfloat16>(c, plan(M, K, F, X, K, W, K, 0, nsm), h);
 }
 
@@ -1395,7 +1401,8 @@ long long g1_gated_ff_workspace(int M, int K, int F, const void* X, long long ld
 int g1_gated_ff(int M, int K, int F, int type, int act, const void* X, long long ldx, const void* W, long long ldw,
                 const float* b, void* h, void* ws, long long ws_size, void* stream) {
     g1ff::Plan L;
-    g1ff::Call c = {M, K, F, type, act, X, M == 1 ? g1ff::pad8(K) : ldx, W, ldw, b, (uint8_t*)ws, (cudaStream_t)stream, 148};
+    g1ff::Call c = {M, K, F, type, act, X, M == 1 ? g1ff::pad8(K) : ldx, W, ldw, b, (uint8_t*)ws, (cudaStream_t)stream, 148,
+                    nullptr};
     const int rc = g1ff::check("g1_gated_ff", M, K, F, type, act, X, c.ldx, W, ldw, b, ws, ws_size, 0, &L, &c.nsm);
     if (rc) return rc;
     if (M > 0 && (!h || ((uintptr_t)h & 1))) { set_error(-22, "g1_gated_ff", "null or misaligned h"); return -22; }
@@ -1409,7 +1416,8 @@ int g1_gated_ff_backward(int M, int K, int F, int type, int act, const void* dh,
                          long long ldw, const float* b, void* dx, void* dw, int dw_type, float* db, void* ws, long long ws_size,
                          void* stream) {
     g1ff::Plan L;
-    g1ff::Call c = {M, K, F, type, act, X, M == 1 ? g1ff::pad8(K) : ldx, W, ldw, b, (uint8_t*)ws, (cudaStream_t)stream, 148};
+    g1ff::Call c = {M, K, F, type, act, X, M == 1 ? g1ff::pad8(K) : ldx, W, ldw, b, (uint8_t*)ws, (cudaStream_t)stream, 148,
+                    nullptr};
     const int rc = g1ff::check("g1_gated_ff_backward", M, K, F, type, act, X, c.ldx, W, ldw, b, ws, ws_size, 1, &L, &c.nsm);
     if (rc) return rc;
     if ((dw_type != 0 && dw_type != type) || ((uintptr_t)dx & 1) || ((uintptr_t)dw & (dw_type == 0 ? 3 : 1)) ||
@@ -1437,9 +1445,13 @@ int g1_gated_ff_test_wait(unsigned limit, void* stream) {
 }
 
 int g1_gated_ff_status(void) {
-    int v = 0, z = 0;
-    if (cudaMemcpyFromSymbol(&v, g1ff::g_err, sizeof v) != cudaSuccess) return -1;
-    if (v && cudaMemcpyToSymbol(g1ff::g_err, &z, sizeof z) != cudaSuccess) return -1;
+    static std::mutex mu;  // g_taken is one a device
+    std::lock_guard<std::mutex> lk(mu);
+    // the calls of every stream are over: those that other threads make from here on are the next status call's
+    if (cudaDeviceSynchronize() != cudaSuccess) return -1;
+    g1ff::k_take_err<<<1, 1>>>();
+    int v = 0;
+    if (cudaGetLastError() != cudaSuccess || cudaMemcpyFromSymbol(&v, g1ff::g_taken, sizeof v) != cudaSuccess) return -1;
     return v;
 }
 

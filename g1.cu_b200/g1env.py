@@ -172,6 +172,7 @@ class G1Env:
             _check()
 
     def tc_status(self):
+        """Nonzero if a wait of this env's tensor-core policy ran out since the last call (waits for the env's stream; clears)."""
         return _lib.g1_env_tc_status(self.h)
 
     def set_value_net(self, hidden=()):
@@ -422,9 +423,13 @@ def gated_ff_backward_device(dh, x, w, b=None, act="silu", need=(True, True, Tru
         return _ff_backward(lib, dev, dh, x, x.shape, b, F, t, code, _ff_operands(x2, w), need, dw_dtype)
 
 
-def gated_ff_status():
-    """Nonzero if a wait inside a gated layer's kernels ran out since the last call (synchronous; clears)."""
-    return load_library().g1_gated_ff_status()
+def gated_ff_status(device=None):
+    """Nonzero if a wait inside a gated layer's kernels ran out on `device` (default: the current one) since the last call, in
+    whatever call but an env's rollout (env.tc_status says that); what they wrote is then garbage.  Waits for all work of
+    the device, so not while a graph is captured; clears."""
+    lib = load_library()
+    with torch.cuda.device(device):
+        return lib.g1_gated_ff_status()
 
 
 class _GatedFF(torch.autograd.Function):

@@ -32,8 +32,8 @@ import torch
 import torch.nn as nn
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
-from g1env import (AC, ClipAdam, G1Env, RunNorm, adv_normalize_device, evaluate, gae_device, obs_prep_device,  # noqa: E402
-                   pack_weights, runnorm_update_device)
+from g1env import (AC, ClipAdam, G1Env, G1Error, RunNorm, adv_normalize_device, evaluate, gae_device,  # noqa: E402
+                   gated_ff_status, obs_prep_device, pack_weights, runnorm_update_device)
 
 
 # ---------------------------------------------------------------- distributed helpers
@@ -113,6 +113,15 @@ def ppo_loss(ac, obs, act, old_logp, adv, ret, clip=0.2, vf_coef=0.5, ent_coef=0
     surrogate = torch.minimum(ratio * adv, ratio.clamp(1.0 - clip, 1.0 + clip) * adv)
     entropy = (log_std + 0.5 + HALF_LOG_2PI).sum(-1)
     return -surrogate.mean() + vf_coef * (val - ret).square().mean() - ent_coef * entropy.mean()
+
+
+def check_waits(env, dev, gated):
+    """Raises if a bounded wait ran out in the rollout or in the gated layers since the last call: trajectories or
+    gradients are then garbage, and so is what the update made of them.  Waits for the device."""
+    if env.tc_status():
+        raise G1Error("a wait of the rollout's tensor-core policy ran out: its outputs are not to be trusted")
+    if gated and gated_ff_status(dev):
+        raise G1Error("a wait of a gated layer ran out: its outputs and gradients are not to be trusted")
 
 
 def ppo_update(ac, opt, b_o, b_a, b_lp, b_adv, b_ret, epochs=5, mb=4, clip=0.2):
@@ -198,6 +207,7 @@ def main():
                           ret.reshape(-1))
         torch.cuda.synchronize()
         t_iter = time.time() - t_it
+        check_waits(env, dev, gated)
         if rank == 0 and config4:
             print(f"iter {it}: wall {t_iter:.3f} s (rollout {t_roll:.3f} s = {world * N * H * 10 / t_roll:.3e} "
                   f"substeps/s, batch prep + PPO update {t_iter - t_roll:.3f} s)", flush=True)
@@ -205,6 +215,7 @@ def main():
         ev = {"fwd_mean": float("nan"), "ep_len_mean": float("nan"), "fall_rate": float("nan"), "vx_mean": float("nan")}
         if rank == 0 and do_eval and ((it % 25 == 0) or it == iters - 1):
             ev = evaluate(env, ac, norm, dev, steps=400 if not smoke else 20)
+            check_waits(env, dev, gated)
             torch.save(dict(model=ac.state_dict(), obs_mean=norm.mean, obs_var=norm.var),
                        os.path.join(out_dir, f"{tag}_last.pt"))
         if rank == 0:

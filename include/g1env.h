@@ -117,8 +117,8 @@ int g1_env_set_policy_ex(void* h, int nh, const int* hidden, int activation, int
  * hidden layers W, b][Wv (1 x last)][bv].  Returns 0 on success. */
 int g1_env_set_value_net(void* h, int nh, const int* hidden);
 
-/* extension: nonzero if a tensor-core wait of the bf16 policy path timed out since the last
- * call (synchronous; clears the flag). */
+/* extension: nonzero if a tensor-core wait of this env's policy (gated layers among it) timed out
+ * since the last call; -1 if that could not be read.  Waits for the env's stream; clears the flag. */
 int g1_env_tc_status(void* h);
 
 /* extension: foot friction coefficient mu of the pyramidal cone (default 0.6). */
@@ -188,8 +188,9 @@ int g1_runnorm_update(int dim, float* mean, float* var, double count, const doub
  * Where rows of X (if M > 4 or backward) or of W do not start on 16-byte boundaries, copies whose rows do (stride K
  * rounded up to 8) are made in it first: X's at its start, W's on the next 256-byte boundary.  A backward call
  * may be given the copies that its forward call left.
- *   g1_gated_ff_status    nonzero if a wait of these kernels ran out on the current device since the last call
- *                         (synchronous; clears) */
+ *   g1_gated_ff_status    nonzero if a wait of these calls ran out on the current device since the last status call (their
+ *                         outputs are then garbage); -1 if that could not be read.  Waits for the device; clears.  Layers
+ *                         in an env's rollout raise that env's flag instead (g1_env_tc_status) */
 long long g1_gated_ff_workspace(int M, int K, int F, const void* X, long long ldx, const void* W, long long ldw,
                                 int backward);
 int g1_gated_ff(int M, int K, int F, int type, int act, const void* X, long long ldx, const void* W, long long ldw,
