@@ -736,8 +736,15 @@ class ClipAdam:
 
     @torch.no_grad()
     def load_state_dict(self, d):
-        if [tuple(m.shape) for m in d["exp_avg"]] != [tuple(p.shape) for p in self.params]:
-            raise G1Error("the state's moments do not have the parameters' shapes")
+        """Takes the state of another ClipAdam over parameters of the same shapes; one that does not fit changes nothing."""
+        for name in ("exp_avg", "exp_avg_sq"):
+            if [tuple(m.shape) for m in d[name]] != [tuple(p.shape) for p in self.params]:
+                raise G1Error("the state's moments do not have the parameters' shapes")
+        steps = torch.as_tensor(d["steps"])
+        if steps.shape != self.steps.shape or steps.dtype != torch.int64 or bool((steps < 0).any()):
+            raise G1Error("the state's steps must be one count a parameter")
+        if torch.as_tensor(d["lr"]).numel() != 1:
+            raise G1Error("the state's lr must be one number")
         if isinstance(self.lr, torch.Tensor):
             self.lr.copy_(torch.as_tensor(d["lr"]).reshape(self.lr.shape))
         else:
@@ -747,7 +754,7 @@ class ClipAdam:
         for ours, theirs in ((self.exp_avg, d["exp_avg"]), (self.exp_avg_sq, d["exp_avg_sq"])):
             for a, b in zip(ours, theirs):
                 a.copy_(b)
-        self.steps.copy_(d["steps"])
+        self.steps.copy_(steps)
 
 
 # ---------------- running obs normalizer (the state of ppo.py:63-81) ----------------

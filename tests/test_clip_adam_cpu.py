@@ -65,3 +65,29 @@ def test_parameter_of_another_shape_is_noticed(make):
     with pytest.raises(g1env.G1Error, match="laid out"):
         opt.step([torch.zeros(2, 3)])
     assert not fake.calls
+
+
+def _state(opt):
+    return [opt.lr] + [t.clone() for t in opt.exp_avg + opt.exp_avg_sq + [opt.steps]]
+
+
+@pytest.mark.parametrize("change", [dict(exp_avg=lambda d: d[:1]), dict(exp_avg_sq=lambda d: d[:1]),
+                                    dict(exp_avg_sq=lambda d: [d[0], d[1][:1]]), dict(exp_avg_sq=lambda d: d + d),
+                                    dict(steps=lambda s: s[:1]), dict(steps=lambda s: torch.tensor(3)),
+                                    dict(steps=lambda s: s - 5), dict(steps=lambda s: s.float()),
+                                    dict(lr=lambda x: torch.ones(2))], ids=lambda c: next(iter(c)))
+def test_a_state_that_does_not_fit_changes_nothing(make, change):
+    """Among them those that broadcasting or a shorter list would have let through."""
+    import g1env
+    ps = lambda: [torch.nn.Parameter(torch.zeros(2, 3)), torch.nn.Parameter(torch.zeros(4))]
+    src, dst = make(ps(), lr=0.5, steps=2)[0], make(ps(), lr=0.1)[0]
+    for t in src.exp_avg + src.exp_avg_sq:
+        t.fill_(1.0)
+    d = src.state_dict()
+    (key, f), = change.items()
+    before = _state(dst)
+    with pytest.raises(g1env.G1Error, match="state"):
+        dst.load_state_dict(dict(d, **{key: f(d[key])}))
+    assert all(torch.equal(a, b) if isinstance(a, torch.Tensor) else a == b for a, b in zip(before, _state(dst)))
+    dst.load_state_dict(d)
+    assert dst.lr == 0.5 and dst.steps.tolist() == [2, 2] and all(bool((t == 1).all()) for t in dst.exp_avg + dst.exp_avg_sq)
