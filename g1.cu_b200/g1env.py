@@ -661,6 +661,8 @@ class ClipAdam:
             for m, p in zip(ms, self.params):
                 if m.shape != p.shape or m.stride() != p.stride():
                     raise G1Error("moments must be laid out like their parameters")
+        if int(steps) < 0:
+            raise G1Error("steps must be >= 0")
         self.steps = torch.full((len(self.params),), int(steps), dtype=torch.int64, device=self.device)
         self._counts = [p.numel() for p in self.params]
         self._shapes = [p.shape for p in self.params]

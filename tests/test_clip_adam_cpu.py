@@ -91,3 +91,9 @@ def test_a_state_that_does_not_fit_changes_nothing(make, change):
     assert all(torch.equal(a, b) if isinstance(a, torch.Tensor) else a == b for a, b in zip(before, _state(dst)))
     dst.load_state_dict(d)
     assert dst.lr == 0.5 and dst.steps.tolist() == [2, 2] and all(bool((t == 1).all()) for t in dst.exp_avg + dst.exp_avg_sq)
+
+
+def test_negative_step_counts_are_refused(make):
+    import g1env
+    with pytest.raises(g1env.G1Error, match="steps"):
+        make([torch.nn.Parameter(torch.zeros(3))], steps=-1)
