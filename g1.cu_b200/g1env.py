@@ -827,9 +827,10 @@ class AC(nn.Module):
         self.log_std = nn.Parameter(-0.5 * torch.ones(act_dim))
 
     def forward(self, x):
-        # gated layers answer in bf16; the heads are fp32
-        z = self.body(x).to(self.mu.weight.dtype)
-        v = self.v(self.v_body(x).to(self.v.weight.dtype)) if self.value_hidden else self.v(z)
+        # gated layers answer in bf16, where the heads are fp32; other layers hand on what they make
+        head = (lambda z: z.to(self.mu.weight.dtype)) if self.activation in ("swiglu", "geglu") else (lambda z: z)
+        z = head(self.body(x))
+        v = self.v(head(self.v_body(x))) if self.value_hidden else self.v(z)
         return self.mu(z), self.log_std.exp(), v.squeeze(-1)
 
 
