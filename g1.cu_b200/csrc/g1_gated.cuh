@@ -6,8 +6,11 @@
 //
 // X, W, h and their gradients are bf16 or fp16, sums and everything between the products fp32; h, dX and dW are
 // rounded once.  dg and du are rounded to the 16-bit type between the two backward products (they are
-// operands of the tensor cores there): half a step of each term, which averages over the sum and stays below
-// the result's own rounding; db is summed from the unrounded values.
+// operands of the tensor cores there).  That is as large an error of dX and dW as rounding the results, independent of it, and it
+// does not average away, as the sums grow like their errors: 2.3e-3 of the norm in bf16 and 2.9e-4 in fp16, where rounding
+// the results alone leaves 1.7e-3 and 2.1e-4; an fp32 dW has no rounding of its own but keeps this one, 1.7e-3 and 2.1e-4.  In
+// fp16 dg and du overflow above 65504, and below 6e-5 they lose digits before dX and dW do: fp32 dW with dh of size 1e-4 is off by
+// 3.1e-4, of size 1e-5 by 2.5e-3, so fp16 rows want a loss scale.  db is summed from the unrounded values.
 //
 // One kernel, k_ff, in several modes, all C = A B with fp32 accumulators in tensor memory, on 256 x 256 tiles by pairs of
 // CTAs (cta_group::2: each CTA loads its 128 rows of A and half of B), or 128 x 128 / 64 by single ones where there

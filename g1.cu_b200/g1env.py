@@ -409,7 +409,9 @@ def gated_ff_device(x, w, b=None, act="silu"):
 def gated_ff_backward_device(dh, x, w, b=None, act="silu", need=(True, True, True), dw_dtype=None):
     """The gradients of gated_ff_device for dh [..., F] (g1_gated_ff_backward): dx like x, dw [2F, K] (dw_dtype: x's type
     or fp32), db [2F] fp32; None where `need` (dx, dw, db) says so.  Nothing of the forward pass but its inputs
-    is needed.  dg and du are rounded to x's type before the products with W and x, but not in db."""
+    is needed.  dg and du are rounded to x's type before the products with W and x, but not in db: dx and dw, an fp32 dw
+    too, carry that rounding of their terms (1.7e-3 of the norm in bf16, 2.1e-4 in fp16).  In fp16 dg and du overflow above
+    65504 and lose digits below 6e-5: scale the loss so that dh lies between."""
     lib = load_library()
     x2, w, b, F, t, code = _ff_args(x, w, b, act)
     dev = x2.device
@@ -471,7 +473,8 @@ _gated_ff_once = torch.autograd.function.once_differentiable(_gated_ff_back)
 
 def gated_ff(x, w, b=None, act="silu"):
     """gated_ff_device with gradients.  w may be fp32 beside 16-bit rows: it is rounded to their type for the
-    products, and its gradient comes back in fp32.  The forward pass keeps only its inputs as the products take them (w
+    products, and its gradient comes back in fp32, summed from terms that are rounded to x's type
+    (gated_ff_backward_device).  The forward pass keeps only its inputs as the products take them (w
     rounded; copies of those whose rows are not on 16-byte boundaries), as saved tensors that hooks and checkpoints see.
     In a captured backward pass the graphs of eager passes over the same leaves have to be gone first, as for any torch
     operator; gated_ff_backward_device has no such tie."""
@@ -482,7 +485,8 @@ def gated_ff(x, w, b=None, act="silu"):
 
 class GatedLinear(nn.Module):
     """A gated layer with fp32 parameters, weight [2F, K] (gate rows, then up rows) and bias [2F], on rows that are taken
-    to `dtype`.  Initialised as nn.Linear(K, 2F)."""
+    to `dtype`.  Initialised as nn.Linear(K, 2F).  The weight's gradient is fp32 with terms rounded to `dtype` (gated_ff); with
+    torch.float16 the loss wants a scale."""
 
     def __init__(self, in_features, out_features, act="silu", bias=True, dtype=torch.bfloat16):
         super().__init__()
