@@ -1837,6 +1837,25 @@ int g1_gemm_bf16_tc(int M, int N, int K, const void* X, int ldx, const void* W, 
 // the last call (synchronises the env's device work; the flag is cleared).
 int g1_env_tc_status(void* h) { return tc_error((EnvState*)h); }
 
+// the numbers in a packed policy (g1_rollout's W) of the env's shape
+long long g1_env_weight_count(void* h) {
+    const EnvState* E = (const EnvState*)h;
+    const int per = E->prec == 1 && E->act >= 2 ? 2 : 1;  // gated layers: W [2h][in], b [2h]
+    long long n = ACT_DIM;                                // log_std
+    auto layers = [&](int nl, const int* hid, int out) {
+        int in = OBS_DIM;
+        for (int l = 0; l < nl; ++l) {
+            n += (long long)per * hid[l] * (in + 1);
+            in = hid[l];
+        }
+        n += (long long)out * (in + 1);
+    };
+    const bool vnet = E->vnh > 0;
+    layers(E->nh, E->hid, ACT_DIM + (vnet ? 0 : 1));
+    if (vnet) layers(E->vnh, E->vhid, 1);
+    return n;
+}
+
 // g1_env.cu:365-382
 void g1_occupancy_report(void) {
     cudaDeviceProp p;

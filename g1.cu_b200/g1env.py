@@ -51,6 +51,7 @@ SIGNATURES = {
     "g1_env_set_friction": (None, [_vp, ctypes.c_float]),
     "g1_env_set_policy_ex": (ctypes.c_int, [_vp, ctypes.c_int, _vp, ctypes.c_int, ctypes.c_int]),
     "g1_env_tc_status": (ctypes.c_int, [_vp]),
+    "g1_env_weight_count": (ctypes.c_longlong, [_vp]),
     "g1_env_set_value_net": (ctypes.c_int, [_vp, ctypes.c_int, _vp]),
     "g1_env_get_state": (None, [_vp, _vp, _vp, _vp, _vp, _vp]),
     "g1_env_set_state": (None, [_vp, _vp, _vp, _vp, _vp, ctypes.c_ulonglong]),
@@ -185,9 +186,19 @@ class G1Env:
     def set_friction(self, mu):
         _lib.g1_env_set_friction(self.h, float(mu))
 
+    def _weights(self, W):
+        """W's address, once it is known to hold all that the env's policy reads (a gated layer's weights are twice a plain
+        one's)."""
+        need = _lib.g1_env_weight_count(self.h)
+        if not W.is_cuda or W.dtype != torch.float32 or not W.is_contiguous():
+            raise G1Error("packed weights must be a contiguous fp32 CUDA tensor")
+        if W.numel() < need:
+            raise G1Error(f"packed weights hold {W.numel()} numbers, the env's policy has {need} (set_policy, set_value_net)")
+        return _dp(W)
+
     def rollout(self, H, W, mean, var, O, A, LP, V, R, D, Vlast):
         """g1_rollout on torch-owned device tensors (ppo_fused.py:101-102)."""
-        _lib.g1_rollout(self.h, H, _dp(W), _dp(mean), _dp(var), _dp(O), _dp(A), _dp(LP), _dp(V), _dp(R), _dp(D),
+        _lib.g1_rollout(self.h, H, self._weights(W), _dp(mean), _dp(var), _dp(O), _dp(A), _dp(LP), _dp(V), _dp(R), _dp(D),
                         _dp(Vlast))
         _check()
 

@@ -117,6 +117,9 @@ int g1_env_set_policy_ex(void* h, int nh, const int* hidden, int activation, int
  * hidden layers W, b][Wv (1 x last)][bv].  Returns 0 on success. */
 int g1_env_set_value_net(void* h, int nh, const int* hidden);
 
+/* extension: how many floats g1_rollout reads from W for the policy and value network that are set. */
+long long g1_env_weight_count(void* h);
+
 /* extension: nonzero if a tensor-core wait of this env's policy (gated layers among it) timed out
  * since the last call; -1 if that could not be read.  Waits for the env's stream; clears the flag. */
 int g1_env_tc_status(void* h);
