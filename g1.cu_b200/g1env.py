@@ -622,8 +622,11 @@ def clip_grad_norm_device(grads, max_norm):
     them.  Tensors of one call may not share memory."""
     lib = load_library()
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    if nn.Parameter in set(map(type, grads)):
+    kinds = set(map(type, grads))
+    if nn.Parameter in kinds:
         raise G1Error("clip_grad_norm_device takes the gradients, not the parameters")
+    if not all(issubclass(t, torch.Tensor) for t in kinds):
+        raise G1Error("gradients must be tensors (leave out those of parameters that have none)")
     dev, kinds = _cuda_list(grads, "gradients", _GRAD_TYPE)
     if dev is None:
         _require_gpu()

@@ -1,4 +1,4 @@
-"""ClipAdam's host side without a GPU: which gradients reach the library.  The library is a fake that keeps the calls; the
+"""The host side of ClipAdam and clip_grad_norm_device without a GPU: which gradients reach the library.  The library is a fake that keeps the calls; the
 tensors are on the CPU, so only the checks of device are out of the way."""
 import contextlib
 
@@ -97,3 +97,12 @@ def test_negative_step_counts_are_refused(make):
     import g1env
     with pytest.raises(g1env.G1Error, match="steps"):
         make([torch.nn.Parameter(torch.zeros(3))], steps=-1)
+
+
+@pytest.mark.parametrize("grads", [[None], [torch.zeros(3), None], ["weight"], {"a": torch.zeros(3)}])
+def test_clipping_says_that_gradients_are_missing(monkeypatch, grads):
+    """A parameter's .grad may be None."""
+    import g1env
+    monkeypatch.setattr(g1env, "load_library", lambda: _Fake())
+    with pytest.raises(g1env.G1Error, match="must be tensors"):
+        g1env.clip_grad_norm_device(grads, 1.0)
