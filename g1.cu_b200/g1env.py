@@ -664,9 +664,13 @@ class ClipAdam:
                  moments=None, steps=0):
         _require_gpu()
         load_library()
+        if isinstance(params, torch.Tensor):
+            raise G1Error("parameters must be a list of tensors")
         self.params = list(params)
         if not self.params:
             raise G1Error("no parameters")
+        if not all(isinstance(p, torch.Tensor) for p in self.params):
+            raise G1Error("parameters must be tensors (no groups of them, no names)")
         self.device = _cuda_list(self.params, "parameters", (torch.float32,))[0]
         self.lr, self.betas, self.eps = lr, (float(betas[0]), float(betas[1])), float(eps)
         self.max_norm, self.weight_decay = float(max_norm), float(weight_decay)

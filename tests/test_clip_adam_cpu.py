@@ -106,3 +106,12 @@ def test_clipping_says_that_gradients_are_missing(monkeypatch, grads):
     monkeypatch.setattr(g1env, "load_library", lambda: _Fake())
     with pytest.raises(g1env.G1Error, match="must be tensors"):
         g1env.clip_grad_norm_device(grads, 1.0)
+
+
+@pytest.mark.parametrize("params", [torch.nn.Parameter(torch.zeros(2, 3)), [{"params": [torch.zeros(3)]}],
+                                    [("w", torch.zeros(3))], [None]], ids=["tensor", "groups", "names", "none"])
+def test_parameters_must_be_a_list_of_tensors(make, params):
+    """One tensor would be taken for the list of its rows, views that nobody else holds."""
+    import g1env
+    with pytest.raises(g1env.G1Error, match="parameters must be"):
+        make(params)
