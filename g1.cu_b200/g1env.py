@@ -445,6 +445,10 @@ def gated_ff_status(device=None):
         return lib.g1_gated_ff_status()
 
 
+def _kind(t):
+    return None if t is None else (t.shape, t.dtype, t.device)
+
+
 class _GatedFF(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, act):
@@ -455,6 +459,7 @@ class _GatedFF(torch.autograd.Function):
         with _on(dev):
             h, ws, nx, nw = _ff_forward(lib, dev, x, x2, w2, b2, F, t, code)
         ctx.save_for_backward(x2, w2, b2, ws)
+        ctx.kinds = [_kind(v) for v in (x2, w2, b2, ws)]
         ctx.call = (lib, dev, F, t, code, nx, nw, x.shape, w.dtype, None if b is None else b.dtype)
         return h
 
@@ -466,9 +471,12 @@ class _GatedFF(torch.autograd.Function):
 
 def _gated_ff_back(ctx, dh):
     # notices a change made since; a hook may have put other tensors in their place
-    x2, w2, b2, ws = ctx.saved_tensors
+    x2, w2, b2, ws = saved = ctx.saved_tensors
+    if [_kind(v) for v in saved] != ctx.kinds:
+        raise G1Error("a hook brought a gated layer's saved tensors back with another shape or type, or on another device")
     lib, dev, F, t, code, nx, nw, shape, w_dtype, b_dtype = ctx.call
     x2, w2 = _rows(x2), _rows(w2)
+    b2, ws = (None if v is None else v.contiguous() for v in (b2, ws))
     operands = _ff_operands(x2, w2)
     if ws is not None:  # the forward pass's copies of unaligned rows
         M, K, px, ldx, pw, ldw = operands
