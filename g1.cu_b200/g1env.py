@@ -683,22 +683,27 @@ class ClipAdam:
         self.lr, self.betas, self.eps = lr, (float(betas[0]), float(betas[1])), float(eps)
         self.max_norm, self.weight_decay = float(max_norm), float(weight_decay)
         like = lambda: [torch.zeros_like(p, requires_grad=False) for p in self.params]
-        self.exp_avg, self.exp_avg_sq = (list(x) for x in moments) if moments is not None else (like(), like())
-        for ms in (self.exp_avg, self.exp_avg_sq):
+        self._m, self._v = (tuple(x) for x in (moments if moments is not None else (like(), like())))
+        for ms in (self._m, self._v):
             if len(ms) != len(self.params):
                 raise G1Error("moments must be one tensor a parameter")
-            _cuda_list(ms + self.params[:1], "moments", (torch.float32,))
+            _cuda_list([*ms, *self.params[:1]], "moments", (torch.float32,))
             for m, p in zip(ms, self.params):
                 if m.shape != p.shape or m.stride() != p.stride():
                     raise G1Error("moments must be laid out like their parameters")
         if int(steps) < 0:
             raise G1Error("steps must be >= 0")
-        self.steps = torch.full((len(self.params),), int(steps), dtype=torch.int64, device=self.device)
+        self._steps = torch.full((len(self.params),), int(steps), dtype=torch.int64, device=self.device)
         self._counts = [p.numel() for p in self.params]
         self._shapes = [p.shape for p in self.params]
         self._strides = [p.stride() for p in self.params]
         self._where = {self.device.index}
-        self._state = self.exp_avg + self.exp_avg_sq + [self.steps]
+        self._state = [*self._m, *self._v, self._steps]
+
+    # the kernel writes to these: their numbers may be changed, the tensors stay
+    exp_avg = property(lambda self: self._m)
+    exp_avg_sq = property(lambda self: self._v)
+    steps = property(lambda self: self._steps)
 
     def zero_grad(self, set_to_none=True):
         for p in self.params:
@@ -750,9 +755,9 @@ class ClipAdam:
             if not (lr.device == dev and lr.dtype == torch.float32 and lr.numel() == 1):
                 raise G1Error("a tensor lr must be one fp32 number on the parameters' device")
             lr, lr_dev = 0.0, lr.data_ptr()
-        p, m, v = _ptrs(params), _ptrs(self.exp_avg), _ptrs(self.exp_avg_sq)
+        p, m, v = _ptrs(params), _ptrs(self._m), _ptrs(self._v)
         with _on(dev):
-            rc = lib.g1_clip_adam(n, _at(ptrs), _at(types), _at(p), _at(m), _at(v), _at(counts), self.steps.data_ptr(),
+            rc = lib.g1_clip_adam(n, _at(ptrs), _at(types), _at(p), _at(m), _at(v), _at(counts), self._steps.data_ptr(),
                                   self.max_norm, lr, lr_dev, self.betas[0], self.betas[1], self.eps, self.weight_decay,
                                   norm.data_ptr(), ws.data_ptr(), size, _stream_of(dev))
         if rc:

@@ -68,7 +68,7 @@ def test_parameter_of_another_shape_is_noticed(make):
 
 
 def _state(opt):
-    return [opt.lr] + [t.clone() for t in opt.exp_avg + opt.exp_avg_sq + [opt.steps]]
+    return [opt.lr] + [t.clone() for t in (*opt.exp_avg, *opt.exp_avg_sq, opt.steps)]
 
 
 @pytest.mark.parametrize("change", [dict(exp_avg=lambda d: d[:1]), dict(exp_avg_sq=lambda d: d[:1]),
@@ -115,3 +115,19 @@ def test_parameters_must_be_a_list_of_tensors(make, params):
     import g1env
     with pytest.raises(g1env.G1Error, match="parameters must be"):
         make(params)
+
+
+def test_the_states_tensors_stay(make):
+    """Other tensors in their places (offloaded, of other lengths) would be written to without a check."""
+    opt, fake = make([torch.nn.Parameter(torch.zeros(2, 3))])
+    was = [opt.exp_avg[0], opt.exp_avg_sq[0], opt.steps]
+    for name in ("exp_avg", "exp_avg_sq", "steps"):
+        with pytest.raises(AttributeError):
+            setattr(opt, name, [torch.zeros(1)])
+    for ms in (opt.exp_avg, opt.exp_avg_sq):
+        with pytest.raises(TypeError):
+            ms[0] = torch.zeros(1)
+    opt.exp_avg[0].fill_(2.0)
+    opt.step([torch.zeros(2, 3)])
+    # n, gradients, types, p, m, v, counts, steps
+    assert fake.calls[0][7] == was[2].data_ptr() and opt.exp_avg[0] is was[0] and opt.exp_avg_sq[0] is was[1]
