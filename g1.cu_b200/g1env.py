@@ -445,8 +445,8 @@ def gated_ff_status(device=None):
         return lib.g1_gated_ff_status()
 
 
-def _kind(t):
-    return None if t is None else (t.shape, t.dtype, t.device)
+def _vector(t, n, dtype, at):
+    return t is None or (t.shape == (n,) and t.dtype == dtype and t.device == at)
 
 
 class _GatedFF(torch.autograd.Function):
@@ -459,8 +459,7 @@ class _GatedFF(torch.autograd.Function):
         with _on(dev):
             h, ws, nx, nw = _ff_forward(lib, dev, x, x2, w2, b2, F, t, code)
         ctx.save_for_backward(x2, w2, b2, ws)
-        ctx.kinds = [_kind(v) for v in (x2, w2, b2, ws)]
-        ctx.call = (lib, dev, F, t, code, nx, nw, x.shape, w.dtype, None if b is None else b.dtype)
+        ctx.call = (lib, dev, F, t, code, nx, nw, x.shape, w.dtype, None if b is None else b.dtype, x2.shape, w2.shape)
         return h
 
     @staticmethod
@@ -471,14 +470,18 @@ class _GatedFF(torch.autograd.Function):
 
 def _gated_ff_back(ctx, dh):
     # notices a change made since; a hook may have put other tensors in their place
-    x2, w2, b2, ws = saved = ctx.saved_tensors
-    if [_kind(v) for v in saved] != ctx.kinds:
+    x2, w2, b2, ws = ctx.saved_tensors
+    lib, dev, F, t, code, nx, nw, shape, w_dtype, b_dtype, rows, cols = ctx.call
+    at, kind = dh.device, dh.dtype  # as the layer's rows had
+    if (x2.shape != rows or w2.shape != cols or x2.dtype != kind or w2.dtype != kind or x2.device != at or w2.device != at
+            or not _vector(b2, 2 * F, torch.float32, at) or not _vector(ws, (nx + nw) // 2, kind, at)):
         raise G1Error("a hook brought a gated layer's saved tensors back with another shape or type, or on another device")
-    lib, dev, F, t, code, nx, nw, shape, w_dtype, b_dtype = ctx.call
     x2, w2 = _rows(x2), _rows(w2)
-    b2, ws = (None if v is None else v.contiguous() for v in (b2, ws))
+    if b2 is not None and not b2.is_contiguous():
+        b2 = b2.contiguous()
     operands = _ff_operands(x2, w2)
     if ws is not None:  # the forward pass's copies of unaligned rows
+        ws = ws.contiguous()
         M, K, px, ldx, pw, ldw = operands
         at, k8 = ws.data_ptr(), (K + 7) & ~7
         operands = (M, K, at if nx else px, k8 if nx else ldx, at + nx if nw else pw, k8 if nw else ldw)
@@ -697,6 +700,7 @@ class ClipAdam:
         self._counts = [p.numel() for p in self.params]
         self._shapes = [p.shape for p in self.params]
         self._strides = [p.stride() for p in self.params]
+        self._flat = all(p.is_contiguous() for p in self.params)
         self._where = {self.device.index}
         self._state = [*self._m, *self._v, self._steps]
 
@@ -712,21 +716,27 @@ class ClipAdam:
             elif p.grad is not None:
                 p.grad.zero_()
 
+    def _like(self, ts):
+        """Whether these lie in memory as the parameters did.  Strides and lengths alone do not say so: [6, 1] and [2, 3] may share
+        strides (3, 1), and only one of them has no gaps."""
+        if [t.shape for t in ts] != self._shapes:
+            return False
+        return all(map(_T.is_contiguous, ts)) if self._flat else list(map(_T.stride, ts)) == self._strides
+
     def step(self, grads=None):
         params, n, dev = self.params, len(self.params), self.device
         grads = [p.grad for p in params] if grads is None else list(grads)
         if len(grads) != n:
             raise G1Error("step takes one gradient (or None) a parameter")
         lib = _lib
-        if (list(map(_T.stride, params)) != self._strides or list(map(_T.size, params)) != self._shapes
-                or set(map(_T.get_device, params)) != self._where or {p.dtype for p in params} != {torch.float32}):
+        if (not self._like(params) or set(map(_T.get_device, params)) != self._where
+                or {p.dtype for p in params} != {torch.float32}):
             raise G1Error("a parameter is no longer laid out as it was when the optimiser was made")
         if any(g is None for g in grads):
             have = [i for i, g in enumerate(grads) if g is not None]
         else:
             have = range(n)
-            # shapes too: [6, 1] and [2, 3] may share strides (3, 1) and lengths, and only one of them has no gaps
-            if list(map(_T.stride, grads)) == self._strides and list(map(_T.size, grads)) == self._shapes:
+            if self._like(grads):
                 have = ()  # nothing to look at one by one
         for i in have:
             g, p = grads[i], params[i]
