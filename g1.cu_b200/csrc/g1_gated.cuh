@@ -36,12 +36,12 @@
 // MMAs, close to the 128 bytes a cycle that it has (tensor pipe 74 % active in DX, 56 % in DZ, whose epilogue moves
 // dh, dg and du through shared memory as well); under the power cap of a long step the clock gives way first.  Below
 // K = 500 or so the epilogues do: 2.7 us a 128 x 128 tile and CTA in FWD, 4.2 us in DZ.
-// Measured on one B200 (graph replays; percent of the measured 1659 TFLOP/s):
-//   forward 32768 x 1024 x 1024              100 us   1370 TFLOP/s   83 %
-//   forward and backward 524288 x 1024 x 512 3.7 to 4.0 ms, by box: FWD 0.80, DZ 0.93, DX 0.82, DW 0.84 each by itself;
-//                                            869 TFLOP/s of the 12MKF that cannot be avoided, 1158 of the 16MKF run
-//   forward 65536 x 104 x 1024               81 us, its DZ 117 us by itself; 151 and 418 MB
-//   forward 1 x 1024 x 1024                  2.0 us   2.1 TB/s from L2: latency
+// Measured on one B200 (graph replays in short bursts; percent of the measured 1659 TFLOP/s):
+//   forward 32768 x 1024 x 1024              98 us    1400 TFLOP/s   84 %; 116 us at length, at 1.40 GHz under the power cap
+//   forward and backward 524288 x 1024 x 512 3.56 ms, 927 TFLOP/s of the 12MKF that cannot be avoided, 1236 of the 16MKF run;
+//                                            4.2 ms at length, at 1.12 GHz.  FWD 0.80, DZ 0.93, DX 0.82, DW 0.84 each by itself
+//   forward 65536 x 104 x 1024               73 us, its DZ 117 us by itself; 151 and 418 MB
+//   forward 1 x 1024 x 1024                  2.5 us   1.7 TB/s from L2: latency
 // Steps: 128-row tiles by single CTAs 117 us and 4.57 ms; pairs of CTAs 109 us and 4.29 ms; coalesced epilogue with
 // two-number arithmetic 101 us and 3.9 ms; accumulators handed back before the stores, no bank conflicts 3.7 ms; DZ alone from
 // 0.98 to 0.93 ms without spills (at K = 104 from 181 to 117 us).
@@ -965,7 +965,7 @@ __global__ void __launch_bounds__(256) k_pad(PadJob a, PadJob b, int ldd, int n)
 // The forward pass of a few rows (a world or some asking for their next action): the weights' bytes are the work, and
 // 128-row tiles would leave it to F / 32 CTAs at most.  One warp an output: it reads row f of Wg and of Wu once, 16 bytes
 // a lane (VEC; single numbers where rows start anywhere), the rows of X come from L1.  R rows at a time.  Measured in a
-// graph, this and 128-row tiles: 1 x 1024 x 1024 2.1 us and 8.1, 4 rows 5.7 and 8.1 (8 rows took 9.9)
+// graph, this and 128-row tiles: 1 x 1024 x 1024 2.1 to 2.5 us and 8.1, 4 rows 5.7 and 8.1 (8 rows took 9.9)
 template <class T, int R, bool VEC>
 __global__ void __launch_bounds__(256) k_ff_rows(int M, int K, int F, int act, const T* X, long long ldx, const T* W, long long ldw,
                                                  const float* bias, T* __restrict__ h) {

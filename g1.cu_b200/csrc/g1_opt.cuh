@@ -31,9 +31,9 @@
 //   clip   99387 fp32 in 9 tensors      7 us (12.4 when each chunk was loaded for the norm and again for the clip)
 //          3e6 bf16 in 300 tensors     14 us; floor 1.8
 //          2.7e8 fp32 in 40 tensors   496 us; floor 328, 491 with the second read that 1 GB needs
-//   Adam   99387                       11 us
-//          2270267 in 17 tensors       15 us; floor 9.7
-//          6.7e7, bf16 gradients      305 us; floor 266, 287 with the second read
+//   Adam   99387                       12 us
+//          2270267 in 17 tensors       14 us; floor 9.7
+//          6.7e7, bf16 gradients      318 to 353 us, by process and box; floor 266, 287 with the second read
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -306,6 +306,7 @@ def dense_bf16x3(X, W, bias=None, act=-1):
 # ---------------- gated layers ----------------
 _ACT = {"tanh": 0, "elu": 1, "silu": 2, "gelu": 3}
 _FF_TYPE = {torch.bfloat16: 1, torch.float16: 2}
+_FF_ROWS = 4  # rows up to which the forward pass makes no copies (g1_gated.cuh ROWS_MAX)
 
 
 _HERE = contextlib.nullcontext()
@@ -375,7 +376,7 @@ def _ff_forward(lib, dev, x, x2, w, b, F, t, code):
     M, K, px, ldx, pw, ldw = _ff_operands(x2, w)
     nx = nw = n = 0
     ws = None
-    if M > 4 and ((px | pw) & 15 or (ldx | ldw) & 7):
+    if M > _FF_ROWS and ((px | pw) & 15 or (ldx | ldw) & 7):
         k8 = (K + 7) & ~7
         nx = (M * k8 * 2 + 255) & ~255 if px & 15 or ldx & 7 else 0
         nw = (F * k8 * 4 + 255) & ~255 if pw & 15 or ldw & 7 else 0

@@ -188,6 +188,7 @@ int g1_runnorm_update(int dim, float* mean, float* var, double count, const doub
  *                         [2F]; any of the three may be NULL.  g and u are computed again from X; dg and du are rounded
  *                         to the inputs' type before their products (not in db; an fp32 dw carries it).  In fp16 they
  *                         overflow above 65504 and lose digits below 6e-5.  Same inputs, same bits.
+ * h, dx, dw and db may share no memory with the inputs or with each other.
  * ws: DEVICE workspace of g1_gated_ff_workspace(...) bytes, 256-byte aligned, for this call alone until it has run.
  * Where rows of X (if M > 4 or backward) or of W do not start on 16-byte boundaries, copies whose rows do (stride K
  * rounded up to 8) are made in it first: X's at its start, W's on the next 256-byte boundary.  A backward call
