@@ -75,6 +75,13 @@ struct Cfg {
     static constexpr int BUF = MODE == DW || MODE == DXS ? 16 : AHEAD * PIECE + (Z ? 1024 : 0);
     static constexpr int STAGE_BYTES = (BM + NB) * BK * 2;
 };
+// The tensor cores truncate: each of the K/16 steps of a sum loses up to a step of fp32 of it, towards 0, so g and u come out
+// smaller the longer the sum.  Of a sum whose terms come in no order a step finds half of it there on the average, and loses about
+// half a step where its terms' bits reach below it: measured on normal x and w, K = 256 to 2048, 0.10 to 0.12 of 2^-23 of the result
+// a step in bf16 and 0.14 in fp16.  DZ puts 1/8 back, as an fma in place of the addition of the bias: db at K = 1024 is off by 5.5e-7 of
+// its norm instead of 1.1e-6, at K = 2048 by 1.2e-6 instead of 2.4e-6.  Sums whose largest terms come first lose twice as much, those
+// whose largest come last a fifth (off by 14 instead of 2 of 2^-23 at K = 2048).  (FWD does not: it rounds h to 16 bits.)
+constexpr float TRUNC = 1.f / (1 << 26);
 constexpr int DW_BLOCK = 64;  // chunks (of 64 rows) that the CTAs of DW walk together
 
 __device__ int g_err;    // a wait of a call that brings no flag of its own ran out
@@ -88,6 +95,7 @@ struct Args {
     const void* dh;              // DZ: [M][F]
     void* out;                   // h [M][F], z [M][2 Fp], dX [M][K], or the fp32 partial tiles
     long long ldo;
+    float2 up;                   // DZ: what an accumulated g or u is multiplied by (see TRUNC)
     float* db;                   // DZ: [gridDim][4][2F] column sums, or null
     int tile0, ntp, blk;         // DW, DXS: the pass's tiles, chunks a block (see Tiles)
     int direct, out32;           // DW: every CTA has the whole sum of its tile: dW itself is written, in fp32 or 16 bits
@@ -366,7 +374,7 @@ __device__ __forceinline__ void fetch4(uint32_t dst, const void* src, bool ok) {
 // z of 32 rows x 16 columns, the s0-th on: dh in `buf` is replaced by dg, du goes to `buf2` (16 columns); the column
 // sums over the rows to sum[k][]: columns 8 k + 2 (l % 4), + 1 of dg, then of du
 template <class T, int ACT, int SC>
-__device__ __forceinline__ void dz16(const uint32_t (&rg)[2][8], const uint32_t (&ru)[2][8], const float (*sb)[32], int s0,
+__device__ __forceinline__ void dz16(const uint32_t (&rg)[2][8], const uint32_t (&ru)[2][8], const float (*sb)[32], const float2& up, int s0,
                                      uint32_t buf, uint32_t buf2, float (&sum)[2][4], int lane) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -380,8 +388,8 @@ __device__ __forceinline__ void dz16(const uint32_t (&rg)[2][8], const uint32_t 
         for (int i = 0; i < 4; ++i) {
             const f2 dh = mk(Half2<T>::unpack(w[i]));
             f2 a, d;
-            act2<ACT, true>(add(acc2(&rg[i / 2][4 * k + 2 * (i & 1)]), bg), a, d);
-            const f2 dg = mul(mul(dh, add(acc2(&ru[i / 2][4 * k + 2 * (i & 1)]), bu)), d), du = mul(dh, a);
+            act2<ACT, true>(fma(acc2(&rg[i / 2][4 * k + 2 * (i & 1)]), mk(up), bg), a, d);
+            const f2 dg = mul(mul(dh, fma(acc2(&ru[i / 2][4 * k + 2 * (i & 1)]), mk(up), bu)), d), du = mul(dh, a);
             const float2 x = un(dg), y = un(du);
             w[i] = Half2<T>::pack(x.x, x.y);
             v[i] = Half2<T>::pack(y.x, y.y);
@@ -808,10 +816,10 @@ __global__ void __launch_bounds__((Cfg<MODE, BN, CG>::NTH), 1) k_ff(const __grid
                             asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
                             if (cc + s + 16 == CW) release();
                             float sum[2][4];
-                            if (P.act == 0) dz16<T, 0, SC>(rg, ru, sb, s, s32(mine), s32(du), sum, lane);
-                            else if (P.act == 1) dz16<T, 1, SC>(rg, ru, sb, s, s32(mine), s32(du), sum, lane);
-                            else if (P.act == 2) dz16<T, 2, SC>(rg, ru, sb, s, s32(mine), s32(du), sum, lane);
-                            else dz16<T, 3, SC>(rg, ru, sb, s, s32(mine), s32(du), sum, lane);
+                            if (P.act == 0) dz16<T, 0, SC>(rg, ru, sb, P.up, s, s32(mine), s32(du), sum, lane);
+                            else if (P.act == 1) dz16<T, 1, SC>(rg, ru, sb, P.up, s, s32(mine), s32(du), sum, lane);
+                            else if (P.act == 2) dz16<T, 2, SC>(rg, ru, sb, P.up, s, s32(mine), s32(du), sum, lane);
+                            else dz16<T, 3, SC>(rg, ru, sb, P.up, s, s32(mine), s32(du), sum, lane);
                             if (P.db) {  // rows behind the last one have dh = 0
 #pragma unroll
                                 for (int k = 0; k < 2; ++k) {
@@ -1225,6 +1233,7 @@ static cudaError_t pair_tiles(const Call& c, Args P, int* ctas) {
         return cudaErrorInvalidValue;
     P.M = c.M; P.N = c.F; P.F = c.F; P.act = c.act; P.bias = c.b; P.err = c.err;
     P.nk = (c.K + BK - 1) / BK;
+    P.up.x = P.up.y = 1.f + TRUNC * (float)((c.K + 15) / 16);
     const int groups = (int)std::min<long long>((long long)((c.M + rows - 1) / rows) * ((c.F + tn - 1) / tn), c.nsm / sh.cg);
     *ctas = groups * sh.cg;
     if (sh.bn == 64) return launch<T, MODE, 64, 1>(P, groups, c.st);

@@ -57,6 +57,26 @@ def test_db_is_summed_before_the_rounding(M, K, F, t):
 
 
 @TYPES
+@pytest.mark.parametrize("K", [512, 1024, 2048])
+def test_long_sums_keep_their_size(K, t):
+    """The tensor cores truncate at each of K/16 steps, which makes sums smaller on the average: half a step of fp32 (0.36 of 2^-23 of
+    the sum, its mantissa being anywhere in [1, 2)) of a sum that is half there on the average, 0.18 of 2^-23 a step at most.  Put
+    back are 2^-26 a step; of what is left, 2^-27 a step is allowed.  One row, dh = 1, ELU and gates above 1/2, where act is
+    g itself: db holds u, then g.  32768 numbers: the mean's own spread is below 2^-27."""
+    import g1env
+    F = 16384
+    g = torch.Generator(device="cuda").manual_seed(K)
+    x = torch.randn(1, K, device="cuda", generator=g).to(t)
+    w = (torch.randn(2 * F, K, device="cuda", generator=g) / math.sqrt(K)).to(t)
+    db = g1env.gated_ff_backward_device(torch.ones(1, F, device="cuda", dtype=t), x, w, None, "elu", (False, False, True))[2].double()
+    z = x[0].double() @ w.double().T
+    far = (z[:F] > 0.5).nonzero()[:, 0]
+    want = torch.cat([z[F:][far], z[:F][far]])
+    off = torch.cat([db[:F][far], db[F:][far]]) - want
+    assert abs((off @ want / (want @ want)).item()) <= 2.0 ** -27 * K / 16
+
+
+@TYPES
 @pytest.mark.parametrize("M,K,F", [(300, 104, 1024), (5000, 40, 24), (10007, 264, 501), (4096, 1024, 512), (130, 60, 33), (64, 1024, 1024)])
 def test_fp32_dw_is_not_rounded_again(M, K, F, t):
     import g1env
